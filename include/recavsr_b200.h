@@ -339,6 +339,53 @@ int rc_cf_wavelet_level(const void* decoded, int dtype, const float* low_c, cons
                         float* blur_r, float* high, uint8_t* out, int T, int H, int W, int radius, int first,
                         int last, rc_stream_t stream);
 
+/* ---- block-scaled FP8 -------------------------------------------------------- */
+/* 8-bit linears with one scale for each block of 128 columns, the finer-grained
+ * form of the per-tensor FP8 linears of recavsr_infer/runtime/fp8.py:13-55.
+ * A matrix [rows, cols] (cols % 16 == 0) is E4M3 codes [rows, cols] and, for
+ * each row's block of 128 columns, an E8M0 scale byte e standing for 2^(e-127):
+ * the smallest e >= 1 with amax <= 448 * 2^(e-127); a block with an infinity or
+ * a NaN has e = 255 and NaN codes. Scale bytes: rc_fp8_block_scales(rows, cols)
+ * bytes in the 128x4 blocked order (128 rows x 4 blocks per 512-byte atom, row
+ * 32 i + j and block k at byte 16 j + 4 i + k), padding zeroed. All pointers
+ * 16-byte aligned unless noted. dtype: 0 fp32, 1 bf16, 2 fp16. Zero rows are
+ * allowed (nothing is launched). */
+long long rc_fp8_block_scales(long long rows, long long cols);
+
+/* Rows x [M, K] (row stride ldx, a multiple of 16 bytes) -> codes, scales. */
+int rc_fp8_block_quantize(const void* x, int dtype, int M, int K, long long ldx, uint8_t* codes,
+                          uint8_t* scales, rc_stream_t stream);
+
+/* Weight w [N, K]: one scale for each 128 x 128 block, stored for each row. */
+int rc_fp8_block_quantize_weight(const void* w, int dtype, int N, int K, long long ldw, uint8_t* codes,
+                                 uint8_t* scales, rc_stream_t stream);
+
+/* RMSNorm rows held in 8 bits (N <= 16384): h = x + residual in fp32, rounded
+ * once into hidden [M, N] (contiguous; residual and hidden both or neither;
+ * hidden == residual is allowed for contiguous rows), y = h * rsqrt(mean(h^2)
+ * + eps) * weight quantized from fp32. */
+int rc_fp8_block_rms_norm(const void* x, long long ldx, const void* residual, long long ldr, int dtype,
+                          int M, int N, const float* weight, float eps, void* hidden, uint8_t* codes,
+                          uint8_t* scales, rc_stream_t stream);
+
+/* out [M, N] = A [M, K] . W [N, K]^T + bias[n] (+ residual), summed in fp32 and
+ * rounded once into out_dtype (1 bf16, 2 fp16; the residual's type too). lda /
+ * ldb in bytes (multiples of 16), ldo / ldr in elements; out and residual need
+ * only their element's alignment (rows on 16 bytes move by TMA), out ==
+ * residual is allowed. bias nullable, fp32. */
+int rc_fp8_block_gemm(const uint8_t* a, long long lda, const uint8_t* a_scales, const uint8_t* b,
+                      long long ldb, const uint8_t* b_scales, const float* bias, int M, int N, int K,
+                      int out_dtype, const void* residual, long long ldr, void* out, long long ldo,
+                      rc_stream_t stream);
+
+/* The gated product of a SwiGLU layer (recavsr_infer/models/flashdecoder/
+ * flashdecoder_wan22.py:344-345) held in 8 bits: y [M, H] = silu(A . Wg^T + bg)
+ * * (A . Wu^T + bu) -> codes, scales. b: ceil(H / 128) groups of 128 gate rows
+ * then 128 up rows (rows past H zero), bias (nullable) in the same order. */
+int rc_fp8_block_swiglu_gemm(const uint8_t* a, long long lda, const uint8_t* a_scales, const uint8_t* b,
+                             long long ldb, const uint8_t* b_scales, const float* bias, int M, int H,
+                             int K, uint8_t* codes, uint8_t* scales, rc_stream_t stream);
+
 /* ---- frame preparation and strip blending -------------------------------- */
 /* Replaces recavsr_infer/video.py:153-179 (`enlarge_block` + `block_tensor`,
  * called by `prepare_block` :138-150): src = `valid` uint8 RGB frames [h, w, 3]

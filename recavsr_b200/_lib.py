@@ -60,10 +60,17 @@ _SIGNATURES = {
     "rc_fd_rope_gather": [_P, _LL] + [_I] * 9 + [_P, _P, _LL, _P, _I, _P, _P, _P, _P],
     "rc_fd_silu": [_P, _I, _I, _I, _P, _P],
     "rc_fd_pixel_shuffle": [_P, _LL, _I, _I, _I, _I, _I, _P, _P],
+    "rc_fp8_block_scales": [_LL, _LL],
+    "rc_fp8_block_quantize": [_P, _I, _I, _I, _LL, _P, _P, _P],
+    "rc_fp8_block_quantize_weight": [_P, _I, _I, _I, _LL, _P, _P, _P],
+    "rc_fp8_block_rms_norm": [_P, _LL, _P, _LL, _I, _I, _I, _P, _F, _P, _P, _P, _P],
+    "rc_fp8_block_gemm": [_P, _LL, _P, _P, _LL, _P, _P, _I, _I, _I, _I, _P, _LL, _P, _LL, _P],
+    "rc_fp8_block_swiglu_gemm": [_P, _LL, _P, _P, _LL, _P, _P, _I, _I, _I, _P, _P, _P],
     "rc_unpatchify_residual": [_P, _LL, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P],
 }
 _RESTYPES = {"rc_paired_attention_workspace": C.c_longlong, "rc_gemm_split_workspace": C.c_longlong,
-             "rc_cross_attention_workspace": C.c_longlong, "rc_cf_adain_workspace": C.c_longlong}
+             "rc_cross_attention_workspace": C.c_longlong, "rc_cf_adain_workspace": C.c_longlong,
+             "rc_fp8_block_scales": C.c_longlong}
 
 _lib = None
 _lock = threading.Lock()
