@@ -83,6 +83,10 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, __half*) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16*) { return rc::pack_bf16x2(a, b); }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ __half from_float(float v, __half*) { return __float2half_rn(v); }
+__device__ __forceinline__ __nv_bfloat16 from_float(float v, __nv_bfloat16*) { return __float2bfloat16_rn(v); }
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
   if constexpr (sizeof(T) == 4) {

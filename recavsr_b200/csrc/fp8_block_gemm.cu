@@ -27,14 +27,16 @@ enum Epi : int { EPI_OUT = 0, EPI_SWIGLU = 1 };
 constexpr int BM = 128;
 constexpr int kRowBytes = 128;        // K elements (bytes) per k-tile: one scale block
 constexpr int kSfAtom = 512;          // 128 rows x 4 scale bytes
-constexpr int kBox = 32 * 128;        // a warp's staging box: 32 rows x 64 16-bit columns
 
 struct Params {
   int M, N, K;                 // N: rows of W
-  int k_tiles, m_blocks, n_blocks, group_m;
+  int k_tiles, m_blocks, n_blocks;
+  int group_m;                 // row blocks per group of the raster
+  uint32_t inv_group, inv_last;   // ceil(2^32 / rows) of a whole and of the last group
   int katoms;                  // scale atoms along K
   const float* bias;           // [N], nullable
-  int staged;                  // OUT: out (and residual) move by TMA
+  int staged;                  // OUT: rows of out (and residual) start on 16 bytes: they move by TMA
+  int pairs;                   // or on 4 bytes
   void* out;                   // OUT
   long long ldo;
   const void* residual;        // OUT, nullable
@@ -61,13 +63,34 @@ struct Smem {
   static constexpr int offA = 0;
   static constexpr int offB = offA + STAGES * kA;
   static constexpr int offOut = offB + STAGES * kB;
-  static constexpr int kOut = EPI == EPI_OUT ? epi_warps<BN>() * kBox : 2 * 4 * 4 * 32 * 4;   // boxes | amax of parts
-  static constexpr int offSf = offOut + kOut;
+  // Staging boxes of a warp's 32 rows, each a TMA store. OUT: 64 columns of 16
+  // bits, or 32 twice where that buys a stage. SWIGLU: 32 codes.
+  static constexpr int kBoxCols = EPI == EPI_SWIGLU ? 32 : BN == 128 ? 64 : 32;
+  static constexpr int kBox = 32 * kBoxCols * (EPI == EPI_SWIGLU ? 1 : 2);
+  static constexpr int kAmax = EPI == EPI_SWIGLU ? 2 * 4 * 4 * 32 * 4 : 0;      // the parts' amax, two tiles
+  static constexpr int kOut = epi_warps<BN>() * kBox + kAmax;
+  static constexpr int offBias = offOut + kOut;                     // 64 fp32 per epilogue warp
+  static constexpr int offSf = offBias + epi_warps<BN>() * 64 * 4;
   static constexpr int offBar = offSf + STAGES * kSf;
   static constexpr int kBars = 2 * STAGES + 6 + 1 + epi_warps<BN>() + 2;
   static constexpr int kTotal = offBar + kBars * 8;
   static_assert(kTotal <= 232448, "shared memory");
 };
+
+__device__ __forceinline__ float4 ld_shared4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint4 ld_shared4u(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ void st_shared4(uint32_t addr, uint4 v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+               : "memory");
+}
 
 template <typename Out>
 __device__ __forceinline__ float2 unpack2(uint32_t w) {
@@ -75,13 +98,51 @@ __device__ __forceinline__ float2 unpack2(uint32_t w) {
   else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 
-// silu(g) * u with the MUFU exp2 and reciprocal (relative error ~1e-6, far
-// below the E4M3 rounding that follows).
+// silu(g) * u with the MUFU exp2 and reciprocal (relative error under 2^-20,
+// far below the E4M3 rounding that follows).
 __device__ __forceinline__ float swiglu(float g, float u) {
   float e, r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
   return g * r * u;
+}
+// 2^z for a pair on the FMA pipe: z = j + f with j = rint(z) and |f| <= 1/2, a
+// degree-5 polynomial for 2^f (coefficients fitted here, relative error
+// 2.1e-7) and j added to the exponent field. z is clamped to [-126, 127]: past
+// either end 1 + 2^z has long become 1, or its reciprocal been flushed to 0.
+__device__ __forceinline__ float2 exp2_fma(float2 z) {
+  constexpr float kRound = 12582912.0f;            // 1.5 * 2^23
+  const float2 zc = make_float2(fminf(fmaxf(z.x, -126.0f), 127.0f), fminf(fmaxf(z.y, -126.0f), 127.0f));
+  const float2 t = __fadd2_rn(zc, make_float2(kRound, kRound));
+  const float2 j = __fadd2_rn(t, make_float2(-kRound, -kRound));
+  const float2 f = __ffma2_rn(j, make_float2(-1.0f, -1.0f), zc);
+  constexpr float c5 = 0.00132764701f, c4 = 0.00967554096f, c3 = 0.0555071346f, c2 = 0.240221202f,
+                  c1 = 0.693146944f, c0 = 1.00000012f;
+  float2 q = __ffma2_rn(make_float2(c5, c5), f, make_float2(c4, c4));
+  q = __ffma2_rn(q, f, make_float2(c3, c3));
+  q = __ffma2_rn(q, f, make_float2(c2, c2));
+  q = __ffma2_rn(q, f, make_float2(c1, c1));
+  q = __ffma2_rn(q, f, make_float2(c0, c0));
+  return make_float2(__uint_as_float(__float_as_uint(q.x) + (__float_as_uint(t.x) << 23)),
+                     __uint_as_float(__float_as_uint(q.y) + (__float_as_uint(t.y) << 23)));
+}
+// silu(g) * u of a pair; the MUFU evaluates the exp2, or (FMA) the polynomial.
+// At two MUFU results per output the MUFU would take as long as the MMAs of a
+// 512-long K, so part of the exp2s run on the FMA pipe.
+template <bool FMA>
+__device__ __forceinline__ float2 swiglu2(float2 g, float2 u) {
+  const float2 z = __fmul2_rn(g, make_float2(-1.4426950408889634f, -1.4426950408889634f));
+  float2 e, r;
+  if constexpr (FMA) {
+    e = exp2_fma(z);
+  } else {
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(z.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(z.y));
+  }
+  const float2 d = __fadd2_rn(e, make_float2(1.0f, 1.0f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(d.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(d.y));
+  return __fmul2_rn(__fmul2_rn(g, r), u);
 }
 
 // Columns of this thread's accumulator row into registers, complete on return.
@@ -97,13 +158,31 @@ __device__ __forceinline__ void acc_ready(uint32_t (&r)[COLS]) {
   for (int c = 0; c < COLS; ++c) asm volatile("" : "+r"(r[c]));   // no use above the wait
 }
 
-__device__ __forceinline__ void tile_coords(const Params& p, int tile, int& mb, int& nb) {
-  const int per_group = p.group_m * p.n_blocks;
-  const int g = tile / per_group, r = tile - g * per_group;
-  const int gm = min(p.group_m, p.m_blocks - g * p.group_m);
-  mb = g * p.group_m + r % gm;
-  nb = r / gm;
-}
+// The tiles of one CTA (or pair), every step-th of the raster: groups of
+// group_m row blocks, row block fastest within a group, then column block, so
+// that one wave's tiles share few operand panels. Walked without a division:
+// every epilogue warp follows it, and its instructions are the epilogue's.
+struct Walk {
+  int r, row0, rows;           // index within the group, the group's first row block and its row blocks
+  __device__ __forceinline__ Walk(const Params& p, int tile) : r(tile), row0(0), rows(min(p.group_m, p.m_blocks)) { settle(p); }
+  __device__ __forceinline__ void settle(const Params& p) {
+    while (r >= rows * p.n_blocks && rows > 0) {
+      r -= rows * p.n_blocks;
+      row0 += rows;
+      rows = min(p.group_m, p.m_blocks - row0);
+    }
+  }
+  __device__ __forceinline__ bool more() const { return rows > 0; }
+  __device__ __forceinline__ void next(const Params& p, int step) {
+    r += step;
+    settle(p);
+  }
+  __device__ __forceinline__ void coords(const Params& p, int& mb, int& nb) const {
+    // r / rows: exact by the reciprocal's high product, as r * rows < 2^32 (checked on the host)
+    nb = rows == 1 ? r : (int)__umulhi((uint32_t)r, rows == p.group_m ? p.inv_group : p.inv_last);
+    mb = row0 + r - nb * rows;
+  }
+};
 
 template <int BN, int STAGES, int EPI, bool PAIR, typename Out>
 __global__ void __launch_bounds__(tile_threads<BN>(), 1)
@@ -185,9 +264,9 @@ tile_kernel(const __grid_constant__ Maps maps, const Params p) {
       uint32_t phase = 0;
       long long issued = 0;
       bool ok = true;
-      for (int tile = tile0; tile < tiles && ok; tile += step) {
+      for (Walk walk(p, tile0); walk.more() && ok; walk.next(p, step)) {
         int mb, nb;
-        tile_coords(p, tile, mb, nb);
+        walk.coords(p, mb, nb);
         const int rb = PAIR ? mb * 2 + (int)rank : mb;                          // this CTA's 128-row block of A
         const int brow = PAIR ? nb * BN + (int)rank * (BN / 2) : nb * BN;       // and its first row of W
         for (int kt = 0; kt < p.k_tiles; ++kt) {
@@ -305,98 +384,178 @@ tile_kernel(const __grid_constant__ Maps maps, const Params p) {
           sm100::mbar_arrive(&acc_empty[as]);
       }
     };
+    float* s_bias = reinterpret_cast<float*>(smem + S::offBias) + w * 64;
+    const uint32_t bias_addr = sm100::smem_u32(s_bias);
     int local = 0;
     uint32_t res_phase = 0;
+    // The bias of the warp's 64 columns passes through shared memory (each lane
+    // loads two and reads all); a tile's is loaded while the tile before it is
+    // waited for, its latency out of the way. So are the tile's coordinates.
+    float bias0 = 0.0f, bias1 = 0.0f;
+    Walk walk(p, tile0);
+    int next_mb = 0, next_nb = 0;
+    auto fetch = [&]() {
+      if (!walk.more()) return;
+      walk.coords(p, next_mb, next_nb);
+      if (!p.bias) return;
+      const int n = next_nb * BN + (EPI == EPI_OUT ? part * 64 : part * 32) + lane, n2 = n + (EPI == EPI_OUT ? 32 : 128);
+      bias0 = n < p.N ? rc::ld_in(p.bias + n) : 0.0f;
+      bias1 = n2 < p.N ? rc::ld_in(p.bias + n2) : 0.0f;
+    };
+    fetch();
     for (int tile = tile0; tile < tiles; tile += step, ++local) {
-      int mb, nb;
-      tile_coords(p, tile, mb, nb);
+      const int mb = next_mb, nb = next_nb;
       const int rb = PAIR ? mb * 2 + (int)rank : mb;
       const int as = local % kAcc;
       const uint32_t parity = (uint32_t)((local / kAcc) & 1);
       const uint32_t tacc = tmem + as * BN + ((uint32_t)(quad * 32) << 16);
       const int row0 = rb * BM + quad * 32, row = row0 + lane;
+      __syncwarp();                            // the last tile's bias has been read
+      s_bias[lane] = bias0;
+      s_bias[32 + lane] = bias1;
+      walk.next(p, step);
+      fetch();
       if constexpr (EPI == EPI_OUT) {
         const int col0 = nb * BN + part * 64;
         const bool inside = row0 < p.M && col0 < p.N;
-        uint8_t* box = smem + S::offOut + w * kBox;
+        uint8_t* box = smem + S::offOut + w * S::kBox;
+        constexpr int kCols = S::kBoxCols;
         const Out* res = static_cast<const Out*>(p.residual);
         Out* out = static_cast<Out*>(p.out);
-        auto at = [&](int r, int c) { return box + sm100::sw128_offset(r, c >> 3) + (c & 7) * 2; };
-        if (p.staged && inside && lane == 0) {
-          sm100::bulk_wait_group_read0();      // the previous tile's store has read the box
-          if (res) {
-            sm100::mbar_arrive_expect_tx(&res_full[w], kBox);
-            sm100::tma_load_2d(box, &maps.res, &res_full[w], col0, row0);
+        // The box's 128- or 64-byte swizzle: 8 lanes' 16-byte granules hit all banks.
+        auto at = [&](int r, int c) {
+          return box + r * (kCols * 2) + (((c >> 3) ^ (kCols == 64 ? r & 7 : (r >> 1) & 3)) << 4) + (c & 7) * 2;
+        };
+        // Rows that do not start on 16 bytes: the warp copies them between the
+        // box and memory, lanes along the columns, in pairs where those are on
+        // 4 bytes; kBatch loads are in flight at a time.
+        const int across = p.pairs ? 2 : 1;
+        constexpr int kBatch = 8;
+        auto copy_in = [&](int h) {
+          const int left = p.N - col0 - h, down = min(32, p.M - row0);
+          const Out* from = res + (size_t)row0 * p.ldr + col0 + h;
+          for (int c = lane * across; c < kCols; c += 32 * across)
+            for (int r0 = 0; r0 < down; r0 += kBatch) {
+              uint32_t v[kBatch];
+#pragma unroll
+              for (int r = 0; r < kBatch; ++r) {
+                v[r] = 0;
+                if (r0 + r < down && c < left) {
+                  const Out* at_r = from + (size_t)(r0 + r) * p.ldr + c;
+                  v[r] = across == 2 && c + 1 < left ? rc::ld_in(reinterpret_cast<const uint32_t*>(at_r))
+                                                    : rc::ld_in(reinterpret_cast<const uint16_t*>(at_r));
+                }
+              }
+#pragma unroll
+              for (int r = 0; r < kBatch; ++r) {
+                if (across == 2) *reinterpret_cast<uint32_t*>(at(r0 + r, c)) = v[r];
+                else *reinterpret_cast<uint16_t*>(at(r0 + r, c)) = (uint16_t)v[r];
+              }
+            }
+        };
+        auto copy_out = [&](int h) {
+          const int left = p.N - col0 - h, down = min(32, p.M - row0);
+          Out* to = out + (size_t)row0 * p.ldo + col0 + h;
+          for (int c = lane * across; c < kCols && c < left; c += 32 * across) {
+#pragma unroll 8
+            for (int r = 0; r < down; ++r) {
+              Out* to_r = to + (size_t)r * p.ldo + c;
+              if (across == 2 && c + 1 < left)
+                *reinterpret_cast<uint32_t*>(to_r) = *reinterpret_cast<const uint32_t*>(at(r, c));
+              else
+                *reinterpret_cast<uint16_t*>(to_r) = *reinterpret_cast<const uint16_t*>(at(r, c));
+            }
           }
+        };
+        auto load_residual = [&](int col) {      // one lane, once the last store has read the box
+          sm100::mbar_arrive_expect_tx(&res_full[w], S::kBox);
+          sm100::tma_load_2d(box, &maps.res, &res_full[w], col, row0);
+        };
+        if (inside) {
+          if (p.staged && lane == 0) {
+            sm100::bulk_wait_group_read0();
+            if (res) load_residual(col0);
+          }
+          if (!p.staged && res) copy_in(0);
         }
-        if (!wait(&acc_full[as], parity, 4)) break;
+        if (!__all_sync(0xffffffffu, wait(&acc_full[as], parity, 4))) break;
         sm100::tc_fence_after();
         uint32_t acc[64];
         load_acc(tacc + part * 64, acc);
         acc_ready(acc);
         release(as);
         if (!inside) continue;
-        if (res) {
+        __syncwarp();
+        bool ok = true;
+#pragma unroll
+        for (int h = 0; h < 64; h += kCols) {
           if (p.staged) {
-            if (!wait(&res_full[w], res_phase, 5)) break;
-            res_phase ^= 1;
-          } else {
-            for (int r = 0; r < 32 && row0 + r < p.M; ++r)
-              for (int c = lane; c < 64 && col0 + c < p.N; c += 32)
-                *reinterpret_cast<Out*>(at(r, c)) = rc::ld_in(res + (size_t)(row0 + r) * p.ldr + col0 + c);
+            if (h) {
+              if (lane == 0) {
+                sm100::bulk_wait_group_read0();
+                if (res) load_residual(col0 + h);
+              }
+              __syncwarp();
+            }
+            if (res) {
+              if (!(ok = __all_sync(0xffffffffu, wait(&res_full[w], res_phase, 5)))) break;
+              res_phase ^= 1;
+            }
+          } else if (res) {
+            if (h) copy_in(h);
             __syncwarp();
           }
-        }
+          // kStep columns at a time, their loads in flight together (as many as the registers hold).
+          constexpr int kStep = BN == 128 ? 16 : 8;
 #pragma unroll
-        for (int g = 0; g < 8; ++g) {
-          const int n = col0 + 8 * g;
-          float v[8];
+          for (int c = 0; c < kCols; c += kStep) {
+            float2 v[kStep / 2];
+            uint4 r[kStep / 8];
+            if (res) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(acc[8 * g + j]);
-          if (p.bias) {
-            if (n + 8 <= p.N) {
-              float b[8];
-              fp8b::load8(p.bias + n, b);
+              for (int i = 0; i < kStep / 8; ++i) r[i] = ld_shared4u(sm100::smem_u32(at(lane, c + 8 * i)));
+            }
 #pragma unroll
-              for (int j = 0; j < 8; ++j) v[j] += b[j];
-            } else {
+            for (int i = 0; i < kStep / 4; ++i) {
+              const float4 b = ld_shared4(bias_addr + (h + c + 4 * i) * 4);
+              v[2 * i] = make_float2(b.x, b.y);
+              v[2 * i + 1] = make_float2(b.z, b.w);
+            }
 #pragma unroll
-              for (int j = 0; j < 8; ++j)
-                if (n + j < p.N) v[j] += rc::ld_in(p.bias + n + j);
+            for (int i = 0; i < kStep / 2; ++i)
+              v[i] = __fadd2_rn(make_float2(__uint_as_float(acc[h + c + 2 * i]),
+                                            __uint_as_float(acc[h + c + 2 * i + 1])), v[i]);
+#pragma unroll
+            for (int i = 0; i < kStep / 8; ++i) {
+              if (res) {
+                v[4 * i] = __fadd2_rn(v[4 * i], unpack2<Out>(r[i].x));
+                v[4 * i + 1] = __fadd2_rn(v[4 * i + 1], unpack2<Out>(r[i].y));
+                v[4 * i + 2] = __fadd2_rn(v[4 * i + 2], unpack2<Out>(r[i].z));
+                v[4 * i + 3] = __fadd2_rn(v[4 * i + 3], unpack2<Out>(r[i].w));
+              }
+              uint32_t o[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) o[j] = fp8b::pack2(v[4 * i + j].x, v[4 * i + j].y, (Out*)nullptr);
+              st_shared4(sm100::smem_u32(at(lane, c + 8 * i)), make_uint4(o[0], o[1], o[2], o[3]));
             }
           }
-          uint4* q = reinterpret_cast<uint4*>(at(lane, 8 * g));
-          if (res) {
-            const uint4 r4 = *q;
-            const uint32_t rw[4] = {r4.x, r4.y, r4.z, r4.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float2 f = unpack2<Out>(rw[j]);
-              v[2 * j] += f.x;
-              v[2 * j + 1] += f.y;
+          if (p.staged) {
+            sm100::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0 && col0 + h < p.N) {
+              sm100::tma_store_2d(&maps.out, box, col0 + h, row0);
+              sm100::bulk_commit_group();
             }
+          } else {
+            __syncwarp();
+            copy_out(h);
+            __syncwarp();                        // the box is free again
           }
-          Out* tag = nullptr;
-          *q = make_uint4(fp8b::pack2(v[0], v[1], tag), fp8b::pack2(v[2], v[3], tag), fp8b::pack2(v[4], v[5], tag),
-                          fp8b::pack2(v[6], v[7], tag));
         }
-        if (p.staged) {
-          sm100::fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            sm100::tma_store_2d(&maps.out, box, col0, row0);
-            sm100::bulk_commit_group();
-          }
-        } else {
-          __syncwarp();
-          for (int r = 0; r < 32 && row0 + r < p.M; ++r)
-            for (int c = lane; c < 64 && col0 + c < p.N; c += 32)
-              out[(size_t)(row0 + r) * p.ldo + col0 + c] = *reinterpret_cast<const Out*>(at(r, c));
-          __syncwarp();                        // the box is free again
-        }
+        if (!ok) break;
       } else {
-        uint32_t* s_amax = reinterpret_cast<uint32_t*>(smem + S::offOut) + ((local & 1) * 4 + quad) * 4 * 32;
-        const bool ok = wait(&acc_full[as], parity, 4);
+        uint32_t* s_amax = reinterpret_cast<uint32_t*>(smem + S::offOut + kEpiWarps * S::kBox) + ((local & 1) * 4 + quad) * 4 * 32;
+        const bool ok = __all_sync(0xffffffffu, wait(&acc_full[as], parity, 4));
         uint32_t acc[64];                      // 32 gate, then the 32 up columns they pair with
         uint32_t m = 0;
         float y[32];
@@ -406,21 +565,31 @@ tile_kernel(const __grid_constant__ Maps maps, const Params p) {
           sm100::tmem_ld32(tacc + 128 + part * 32, acc + 32);
           acc_ready(acc);
           release(as);
+          __syncwarp();
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            float bg[8] = {}, bu[8] = {};
-            const int n = nb * BN + part * 32 + 8 * g;
-            if (p.bias) {
-              fp8b::load8(p.bias + n, bg);
-              fp8b::load8(p.bias + n + 128, bu);
-            }
+          for (int c = 0; c < 32; c += 4) {
+            const float4 bg = ld_shared4(bias_addr + c * 4), bu = ld_shared4(bias_addr + (32 + c) * 4);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float v = swiglu(__uint_as_float(acc[8 * g + j]) + bg[j], __uint_as_float(acc[32 + 8 * g + j]) + bu[j]);
-              y[8 * g + j] = nb * 128 + part * 32 + (8 * g & ~15) < p.H ? v : 0.0f;
-              m = max(m, fp8b::magnitude(y[8 * g + j]));
+            for (int i = 0; i < 4; i += 2) {
+              const float2 g = __fadd2_rn(make_float2(__uint_as_float(acc[c + i]), __uint_as_float(acc[c + i + 1])),
+                                          i ? make_float2(bg.z, bg.w) : make_float2(bg.x, bg.y));
+              const float2 u = __fadd2_rn(make_float2(__uint_as_float(acc[32 + c + i]), __uint_as_float(acc[33 + c + i])),
+                                          i ? make_float2(bu.z, bu.w) : make_float2(bu.x, bu.y));
+              const float2 v = i == 2 && c % 8 == 4 ? swiglu2<true>(g, u) : swiglu2<false>(g, u);
+              y[c + i] = v.x;
+              y[c + i + 1] = v.y;
             }
           }
+          const int left = p.H - nb * 128 - part * 32;      // columns of this part that exist: none, 16 or 32
+          if (left < 32) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              if (c >= 16 || left < 16) y[c] = 0.0f;
+          }
+          float top = 0.0f;
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) top = rc::absmax3_nan(top, y[c], y[c + 1]);
+          m = fp8b::magnitude(top);
           s_amax[part * 32 + lane] = m;
         }
         // The four warps of a lane quadrant share its rows' amax. (The buffer
@@ -429,25 +598,35 @@ tile_kernel(const __grid_constant__ Maps maps, const Params p) {
         m = max(max(s_amax[lane], s_amax[32 + lane]), max(s_amax[64 + lane], s_amax[96 + lane]));
         const uint32_t e = fp8b::scale_byte(m);
         const float inv = fp8b::inverse_scale(e);
+        // A store from registers would touch 32 rows per instruction: the codes
+        // leave by TMA from a box of 32 rows x 32 bytes.
         const int col0 = nb * 128 + part * 32;
-        if (row < p.M) {
-          uint32_t c[8];
+        uint8_t* box = smem + S::offOut + w * S::kBox;
+        if (lane == 0) sm100::bulk_wait_group_read0();     // the last tile's store has read it
+        __syncwarp();
+        uint32_t c[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            c[j] = fp8b::e4m3x4(y[4 * j] * inv, y[4 * j + 1] * inv, y[4 * j + 2] * inv, y[4 * j + 3] * inv);
-          uint4* dst = reinterpret_cast<uint4*>(p.codes + (size_t)row * p.H + col0);
-          if (col0 < p.H) dst[0] = make_uint4(c[0], c[1], c[2], c[3]);
-          if (col0 + 16 < p.H) dst[1] = make_uint4(c[4], c[5], c[6], c[7]);
+        for (int j = 0; j < 8; ++j)
+          c[j] = fp8b::e4m3x4(y[4 * j] * inv, y[4 * j + 1] * inv, y[4 * j + 2] * inv, y[4 * j + 3] * inv);
+        const uint32_t dst = sm100::smem_u32(box) + lane * 32;
+        st_shared4(dst, make_uint4(c[0], c[1], c[2], c[3]));
+        st_shared4(dst + 16, make_uint4(c[4], c[5], c[6], c[7]));
+        sm100::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0 && row0 < p.M && col0 < p.H) {
+          sm100::tma_store_2d(&maps.out, box, col0, row0);
+          sm100::bulk_commit_group();
         }
         if (part == 0 && row < (p.M + 127) / 128 * 128) {
           const int atoms = fp8b::atoms_of(p.H);
-          p.scales[rc::sf_offset(row, nb, atoms)] = row < p.M ? (uint8_t)e : 0;
+          uint8_t* at = p.scales + ((size_t)rb * atoms + (nb >> 2)) * kSfAtom + lane * 16 + quad * 4;   // rc::sf_offset
+          at[nb & 3] = row < p.M ? (uint8_t)e : 0;
           if (nb == p.n_blocks - 1)
-            for (int kb = p.n_blocks; kb < 4 * atoms; ++kb) p.scales[rc::sf_offset(row, kb, atoms)] = 0;
+            for (int kb = (nb & 3) + 1; kb < 4; ++kb) at[kb] = 0;
         }
       }
     }
-    if (EPI == EPI_OUT && lane == 0) sm100::bulk_wait_group0();
+    if (lane == 0) sm100::bulk_wait_group0();
   }
   sm100::tc_fence_before();
   __syncthreads();
@@ -478,30 +657,411 @@ int launch(const Maps& maps, const Params& p, cudaStream_t stream, const char* w
       rc::launch_pdl(kern, dim3(tiles < sms ? tiles : sms), dim3(tile_threads<BN>()), S::kTotal, stream, maps, p), what);
 }
 
+// Four columns n .. n+3 of an output row: bias and residual (`near`, loaded
+// ahead where rows start on 16 bytes) added, rounded, stored.
+template <typename Out>
+__device__ __forceinline__ void store_piece(const Params& p, int row, int n, const float (&sum)[4], uint2 near) {
+  const Out* res = static_cast<const Out*>(p.residual);
+  Out* out = static_cast<Out*>(p.out) + (size_t)row * p.ldo + n;
+  float f[4] = {sum[0], sum[1], sum[2], sum[3]};
+  if (p.bias) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (n + c < p.N) f[c] += rc::ld_in(p.bias + n + c);
+  }
+  if (p.staged && n + 4 <= p.N) {
+    if (res) {
+      const float2 lo = unpack2<Out>(near.x), hi = unpack2<Out>(near.y);
+      f[0] += lo.x;
+      f[1] += lo.y;
+      f[2] += hi.x;
+      f[3] += hi.y;
+    }
+    Out* tag = nullptr;
+    *reinterpret_cast<uint2*>(out) = make_uint2(fp8b::pack2(f[0], f[1], tag), fp8b::pack2(f[2], f[3], tag));
+  } else {
+    float r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (res) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (n + c < p.N) r[c] = fp8b::to_float(rc::ld_in(res + (size_t)row * p.ldr + n + c));
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (n + c < p.N) out[c] = fp8b::from_float(f[c] + r[c], (Out*)nullptr);
+  }
+}
+
+// ---------------------------------------------------------------- few rows
+// The same products with the operands' roles exchanged, for outputs of too few
+// 128 x 128 tiles to fill the GPU: W's 128 rows are the MMA's M side and the
+// BT (16 or 32) rows of A its N side, so a single row of A costs a 16-column
+// MMA; and a cluster of up to 8 CTAs splits K. Each CTA accumulates its k-tiles
+// in TMEM and pushes its fp32 partial, row of A by row, into the shared memory
+// of the CTA that owns the row (stores do not wait for the other SM, reads
+// would); after a cluster barrier each CTA sums its rows' partials in rank
+// order (a fixed order: equal inputs give equal bits) and runs the epilogue,
+// one warp per row, four columns per lane. SWIGLU runs a gate and an up tile
+// side by side (kW = 2): a row's 128 outputs are one warp's, so the block's
+// amax is one warp reduction.
+constexpr int kRowsThreads = 192;     // producer, MMA issuer, 4 TMEM warps; all 6 in the epilogue
+
+template <int BT, int EPI>
+struct RowsSmem {
+  static constexpr int kW = EPI == EPI_SWIGLU ? 2 : 1;
+  static constexpr int kStage = (kW * BM + BT) * kRowBytes;
+  static constexpr int kSf = (kW + 1) * kSfAtom;
+  static constexpr int kStages = 98304 / (kStage + kSf);    // two CTAs per SM where they fit
+  static constexpr int kPart = kW * (BT + 8) * BM * 4;      // the partials of the rows this CTA owns, by rank
+  static constexpr int offPart = kStages * kStage;
+  static constexpr int offSf = offPart + kPart;
+  static constexpr int offBar = offSf + kStages * kSf;
+  static constexpr int kTotal = offBar + (2 * kStages + 3) * 8;
+  static constexpr int kTmem = kW * BT + 2 * 4 * (kW + 1);
+  static constexpr int kTmemCols = kTmem <= 32 ? 32 : kTmem <= 64 ? 64 : kTmem <= 128 ? 128 : kTmem <= 256 ? 256 : 512;
+  static_assert(kTotal <= 232448, "shared memory");
+};
+
+template <int BT, int EPI, typename Out>
+__global__ void __launch_bounds__(kRowsThreads)
+rows_kernel(const __grid_constant__ Maps maps, const Params p, int split) {
+  using S = RowsSmem<BT, EPI>;
+  constexpr int kW = S::kW, STAGES = S::kStages;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::offBar);
+  uint64_t* empty = full + STAGES;
+  uint64_t* acc_full = empty + STAGES;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(acc_full + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 2);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = (int)sm100::cluster_ctarank();
+  const int tile = blockIdx.x / split;
+  const int tt = tile % p.m_blocks, wt = tile / p.m_blocks;     // tiles of one W block are neighbours
+  const int kt0 = (int)((long long)rank * p.k_tiles / split), kt1 = (int)((long long)(rank + 1) * p.k_tiles / split);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      sm100::mbar_init(&full[s], 1);
+      sm100::mbar_init(&empty[s], 1);
+    }
+    sm100::mbar_init(acc_full, 1);
+    *abort_flag = 0;
+    sm100::fence_mbar_init();
+  }
+  if (warp == 1) {
+    sm100::tmem_alloc(tmem_slot, S::kTmemCols);
+    sm100::tmem_relinquish();
+  }
+  sm100::tc_fence_before();
+  __syncthreads();
+  sm100::tc_fence_after();
+  rc::pdl_trigger();
+  rc::pdl_wait();
+  const uint32_t tmem = *tmem_slot, tmem_sf = tmem + kW * BT;
+  auto wait = [&](uint64_t* bar, uint32_t parity, unsigned int site) -> bool {
+    if (sm100::mbar_wait(bar, parity, abort_flag)) return true;
+    if (!*abort_flag) {
+      rc::device_fail(kKernFp8Block, site);
+      *abort_flag = 1;
+    }
+    return false;
+  };
+
+  if (warp == 0) {
+    if (sm100::elect_one_sync()) {
+      int stage = 0, issued = 0;
+      uint32_t phase = 0;
+      for (int kt = kt0; kt < kt1; ++kt) {
+        if (!wait(&empty[stage], phase ^ 1, 11)) break;
+        uint8_t* a = smem + stage * S::kStage;
+        uint8_t* sf = smem + S::offSf + stage * S::kSf;
+        const bool atom = (kt & 3) == 0 || kt == kt0;
+        const int line = (kt >> 2) * 4;
+        sm100::mbar_arrive_expect_tx(&full[stage], S::kStage + (atom ? S::kSf : 0));
+#pragma unroll
+        for (int w = 0; w < kW; ++w)
+          sm100::tma_load_2d(a + w * BM * kRowBytes, &maps.b, &full[stage], kt * kRowBytes, (wt * kW + w) * BM);
+        sm100::tma_load_2d(a + kW * BM * kRowBytes, &maps.a, &full[stage], kt * kRowBytes, tt * BT);
+        if (atom) {
+#pragma unroll
+          for (int w = 0; w < kW; ++w)
+            sm100::tma_load_2d(sf + w * kSfAtom, &maps.sfb, &full[stage], 0, (wt * kW + w) * p.katoms * 4 + line);
+          sm100::tma_load_2d(sf + kW * kSfAtom, &maps.sfa, &full[stage], 0, tt * BT / 128 * p.katoms * 4 + line);
+        }
+        ++issued;
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+      }
+      for (int s = 0; s < STAGES && issued > 0; ++s, --issued) {   // loads land before the CTA goes on
+        if (stage == 0) { stage = STAGES; phase ^= 1; }
+        --stage;
+        sm100::mbar_wait(&full[stage], phase);
+      }
+    }
+  } else if (warp == 1) {
+    if (sm100::elect_one_sync()) {
+      int stage = 0, sf_buf = 1;
+      uint32_t phase = 0, sfw = 0;
+      const uint64_t d0 = sm100::desc_kmajor_sw128(sm100::smem_u32(smem));
+      const uint64_t dsf0 = sm100::desc_sf_rows(sm100::smem_u32(smem + S::offSf));
+      for (int kt = kt0; kt < kt1; ++kt) {
+        if (!wait(&full[stage], phase, 12)) break;
+        sm100::tc_fence_after();
+        if ((kt & 3) == 0 || kt == kt0) {
+          sf_buf ^= 1;
+          sfw = tmem_sf + sf_buf * 4 * (kW + 1);
+#pragma unroll
+          for (int w = 0; w <= kW; ++w)
+            sm100::tmem_cp_32x128b_warpx4(sfw + 4 * w, sm100::desc_add(dsf0, stage * S::kSf + w * kSfAtom));
+        }
+        const uint32_t idesc = sm100::idesc_mxf8(BM, BT, 0) | ((kt & 3) << 4) | ((kt & 3) << 29);
+        const uint64_t da = sm100::desc_add(d0, stage * S::kStage);
+        const uint64_t db = sm100::desc_add(da, kW * BM * kRowBytes);
+#pragma unroll
+        for (int w = 0; w < kW; ++w)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            sm100::mma_mxf8_ss(tmem + w * BT, sm100::desc_add(da, w * BM * kRowBytes + 32 * j),
+                               sm100::desc_add(db, 32 * j), idesc, sfw + 4 * w, sfw + 4 * kW, kt != kt0 || j != 0);
+        sm100::tc_commit(&empty[stage]);
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+      }
+      sm100::tc_commit(acc_full);
+      sm100::mbar_wait(acc_full, 0);
+    }
+  }
+  __syncwarp();
+  const int rows = min(BT, p.M - tt * BT), per = (rows + split - 1) / split;   // rank q owns rows q * per ...
+  float* part = reinterpret_cast<float*>(smem + S::offPart);    // [rank][kW][per][128]
+  bool ok = true;
+  if (warp >= 2) {
+    ok = __all_sync(0xffffffffu, wait(acc_full, 0, 13));
+    sm100::tc_fence_after();
+  }
+  if (warp >= 2 && ok) {
+    const int quad = warp & 3;
+    constexpr int kChunk = BT < 32 ? BT : 32;
+    const uint32_t mine = sm100::smem_u32(part) + (rank * kW * per * BM + quad * 32 + lane) * 4;
+#pragma unroll
+    for (int w = 0; w < kW; ++w) {
+      int owner = 0, i = 0;
+      uint32_t to = sm100::mapa(mine + w * per * BM * 4, 0);
+      for (int c = 0; c < BT; c += kChunk) {
+        if (c >= rows) break;
+        uint32_t acc[kChunk];
+        const uint32_t addr = tmem + w * BT + c + ((uint32_t)(quad * 32) << 16);
+        if constexpr (kChunk == 16) sm100::tmem_ld16(addr, acc);
+        else sm100::tmem_ld32(addr, acc);
+        acc_ready(acc);
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) {
+          if (c + j >= rows) break;
+          asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(to), "r"(acc[j]) : "memory");
+          to += BM * 4;
+          if (++i == per) {
+            i = 0;
+            ++owner;
+            to = sm100::mapa(mine + w * per * BM * 4, min(owner, split - 1));
+          }
+        }
+      }
+    }
+    sm100::tc_fence_before();
+  }
+  sm100::cluster_sync();
+  if (warp == 1) {
+    sm100::tc_fence_after();
+    sm100::tmem_dealloc(tmem, S::kTmemCols);
+  }
+  // A warp takes kRows of this CTA's rows at a time, their loads in flight together.
+  const int first = rank * per, mine = min(per, rows - first);
+  constexpr int kRows = BT / 16;
+  float4 bias[kW];
+  if (p.bias) {
+#pragma unroll
+    for (int w = 0; w < kW; ++w) {
+      const int n = (wt * kW + w) * BM + lane * 4;
+      bias[w].x = n < p.N ? rc::ld_in(p.bias + n) : 0.0f;
+      bias[w].y = n + 1 < p.N ? rc::ld_in(p.bias + n + 1) : 0.0f;
+      bias[w].z = n + 2 < p.N ? rc::ld_in(p.bias + n + 2) : 0.0f;
+      bias[w].w = n + 3 < p.N ? rc::ld_in(p.bias + n + 3) : 0.0f;
+    }
+  } else {
+#pragma unroll
+    for (int w = 0; w < kW; ++w) bias[w] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  }
+  for (int i = warp * kRows; i < mine; i += kRowsThreads / 32 * kRows) {
+    float4 v[kRows][kW];
+#pragma unroll
+    for (int j = 0; j < kRows; ++j)
+#pragma unroll
+      for (int w = 0; w < kW; ++w) v[j][w] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    uint2 near[kRows];                                             // residual
+    const Out* res = static_cast<const Out*>(p.residual);
+    const int n = wt * BM + lane * 4;
+    const bool vec = p.staged && n + 4 <= p.N;
+    if (EPI == EPI_OUT && res && vec) {
+#pragma unroll
+      for (int j = 0; j < kRows; ++j)
+        near[j] = rc::ld_in(reinterpret_cast<const uint2*>(
+            res + (size_t)(tt * BT + first + min(i + j, mine - 1)) * p.ldr + n));
+    }
+    for (int q = 0; q < split; ++q) {
+#pragma unroll
+      for (int j = 0; j < kRows; ++j)
+#pragma unroll
+        for (int w = 0; w < kW; ++w) {
+          // past the last row: the last once more, not stored
+          const float4 x = ld_shared4(sm100::smem_u32(part) + (((q * kW + w) * per + min(i + j, mine - 1)) * BM + lane * 4) * 4);
+          v[j][w].x += x.x;
+          v[j][w].y += x.y;
+          v[j][w].z += x.z;
+          v[j][w].w += x.w;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) {
+      if (i + j >= mine) break;
+      const int row = tt * BT + first + i + j;
+#pragma unroll
+      for (int w = 0; w < kW; ++w) {
+        v[j][w].x += bias[w].x;
+        v[j][w].y += bias[w].y;
+        v[j][w].z += bias[w].z;
+        v[j][w].w += bias[w].w;
+      }
+      if constexpr (EPI == EPI_OUT) {
+        Out* out = static_cast<Out*>(p.out) + (size_t)row * p.ldo + n;
+        float f[4] = {v[j][0].x, v[j][0].y, v[j][0].z, v[j][0].w};
+        if (vec) {
+          if (res) {
+            const float2 lo = unpack2<Out>(near[j].x), hi = unpack2<Out>(near[j].y);
+            f[0] += lo.x;
+            f[1] += lo.y;
+            f[2] += hi.x;
+            f[3] += hi.y;
+          }
+          Out* tag = nullptr;
+          *reinterpret_cast<uint2*>(out) = make_uint2(fp8b::pack2(f[0], f[1], tag), fp8b::pack2(f[2], f[3], tag));
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (n + c < p.N) {
+              if (res) f[c] += fp8b::to_float(rc::ld_in(res + (size_t)row * p.ldr + n + c));
+              out[c] = fp8b::from_float(f[c], (Out*)nullptr);
+            }
+        }
+      } else {
+        const float g[4] = {v[j][0].x, v[j][0].y, v[j][0].z, v[j][0].w};
+        const float u[4] = {v[j][kW - 1].x, v[j][kW - 1].y, v[j][kW - 1].z, v[j][kW - 1].w};
+        float y[4];
+        const int col = wt * 128 + lane * 4;
+        uint32_t m = 0;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          y[c] = col < p.H ? swiglu(g[c], u[c]) : 0.0f;      // H is a multiple of 16
+          m = max(m, fp8b::magnitude(y[c]));
+        }
+        const uint32_t e = fp8b::scale_byte(__reduce_max_sync(0xffffffffu, m));
+        const float inv = fp8b::inverse_scale(e);
+        if (col < p.H)
+          *reinterpret_cast<uint32_t*>(p.codes + (size_t)row * p.H + col) =
+              fp8b::e4m3x4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
+        if (lane == 0) p.scales[rc::sf_offset(row, wt, fp8b::atoms_of(p.H))] = (uint8_t)e;
+      }
+    }
+  }
+  if constexpr (EPI == EPI_SWIGLU) {
+    // Zero scales: rows past M of this tile's 128 (or BT, the only tile), and
+    // the last block's neighbours up to the atom.
+    const int atoms = fp8b::atoms_of(p.H), last = (p.M + 127) / 128 * 128;
+    if (rank == 0)
+      for (int row = tt * 128 + threadIdx.x; row < min(tt * 128 + 128, last); row += kRowsThreads) {
+        if (row >= p.M) p.scales[rc::sf_offset(row, wt, atoms)] = 0;
+        if (wt == p.n_blocks - 1)
+          for (int kb = p.n_blocks; kb < 4 * atoms; ++kb) p.scales[rc::sf_offset(row, kb, atoms)] = 0;
+      }
+  }
+}
+
+template <int BT, int EPI, typename Out>
+int launch_rows(const Maps& maps, const Params& p, int split, cudaStream_t stream, const char* what) {
+  using S = RowsSmem<BT, EPI>;
+  auto kern = rows_kernel<BT, EPI, Out>;
+  static rc::SmemAttrFlags flags = {};
+  if (const int r = rc::ensure_smem_attr(flags, reinterpret_cast<const void*>(kern), S::kTotal, what)) return r;
+  return rc::check_launch(rc::launch_pdl_cluster(kern, dim3((unsigned)(p.m_blocks * p.n_blocks * split)),
+                                                 dim3(kRowsThreads), S::kTotal, stream, (unsigned)split, maps, p, split),
+                          what);
+}
+
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-// Checks and tensor maps the two products share. rows of W: N; its first
-// 128-row block's scales start at sb.
+// How a product runs.
+struct Plan {
+  int bt;        // rows kernel with BT rows of A per tile; 0: tile kernel
+  int split;     // rows kernel: CTAs per tile along K
+  int bn;        // tile kernel: columns per tile
+  bool pair;     // tile kernel: CTA pairs (256 x 256 tiles)
+};
+
+// Up to 32 rows run on the rows kernel, K split until two CTAs per SM have
+// work (measured, B200, us, split 1 / 2 / 4 / 8: 1 x 512 x 512 3.3 / 3.0 / 2.8
+// / -, 1 x 3072 x 3072 - / 4.9 / 4.1 / 4.2, 24 x 3072 x 14336 - / - / 14.0 /
+// 11.1; the tile kernel 4.1, 7.1 and 33). More rows take the tile kernel whose
+// waves cost less. Cycles of a k-tile and of a tile's hand-off, measured with
+// every SM busy: 400 and 300 on 128 x 128 tiles, 520 and 1300 on pairs, 620
+// and 1300 on 128 x 256, and 1500, 3000, 3000 for the last tile's epilogue
+// (3520 x 768 x 512: 5.0 us on 128 x 128 against 6.3 on pairs; 7040 x 3072 x
+// 3072 59 against 69 the other way).
+Plan plan_for(int M, int N, int K, bool swiglu) {
+  const int sms = rc::sm_count(), k_tiles = fp8b::blocks_of(K);
+  auto up = [](long long a, long long b) { return (a + b - 1) / b; };
+  Plan q{0, 1, 256, false};
+  if (M <= 32) {
+    q.bt = M <= 16 ? 16 : 32;
+    const long long room = 2LL * sms / up(N, swiglu ? 256 : 128);
+    q.split = (int)(room < 1 ? 1 : room > 8 ? 8 : room);
+    if (q.split > k_tiles) q.split = k_tiles;
+    return q;
+  }
+  const long long pair = up(up(M, 256) * up(N, 256), sms / 2) * (520LL * k_tiles + 1300) + 3000;
+  const long long one = swiglu ? up(up(M, 128) * up(N, 256), sms) * (620LL * k_tiles + 1300) + 3000
+                               : up(up(M, 128) * up(N, 128), sms) * (400LL * k_tiles + 300) + 1500;
+  q.pair = pair < one;
+  if (!q.pair && !swiglu) q.bn = 128;
+  return q;
+}
+
+// Tensor maps the two products share. N: rows of W.
 int prepare(const char* what, const void* a, long long lda, const void* sa, const void* b, long long ldb,
-            const void* sb, int M, int N, int K, int bn, bool pair, Params& p, Maps& maps) {
+            const void* sb, int M, int N, int K, bool swiglu, const Plan& q, Params& p, Maps& maps) {
+  const int rows_a = q.bt ? q.bt : BM, rows_b = q.bt ? BM : q.pair ? q.bn / 2 : q.bn;   // TMA boxes
+  const int tile_m = q.bt ? q.bt : q.pair ? 2 * BM : BM, tile_n = q.bt ? (swiglu ? 256 : 128) : q.bn;
   p.M = M;
   p.N = N;
   p.K = K;
   p.k_tiles = fp8b::blocks_of(K);
   p.katoms = fp8b::atoms_of(K);
-  p.m_blocks = (M + (pair ? 2 * BM : BM) - 1) / (pair ? 2 * BM : BM);
-  p.n_blocks = (N + bn - 1) / bn;
-  p.group_m = p.m_blocks;
+  p.m_blocks = (M + tile_m - 1) / tile_m;
+  p.n_blocks = (N + tile_n - 1) / tile_n;
+  // A wave of (pairs of) SMs takes a group of row blocks times as many column
+  // blocks as are left: near to square, it touches the fewest operand panels.
+  p.group_m = q.pair ? 8 : 12;
+  if (p.group_m > p.m_blocks) p.group_m = p.m_blocks;
+  const int last = p.m_blocks % p.group_m ? p.m_blocks % p.group_m : p.group_m;
+  p.inv_group = (uint32_t)((0x100000000ull + p.group_m - 1) / p.group_m);
+  p.inv_last = (uint32_t)((0x100000000ull + last - 1) / last);
   const long long lines_a = 4LL * p.katoms * ((M + 127) / 128), lines_b = 4LL * p.katoms * ((N + 127) / 128);
-  if ((long long)p.m_blocks * p.n_blocks > INT32_MAX || lines_a > INT32_MAX || lines_b > INT32_MAX)
+  if ((long long)p.m_blocks * p.n_blocks * q.split > INT32_MAX || p.n_blocks > (1 << 24) || lines_a > INT32_MAX || lines_b > INT32_MAX)
     return rc::set_error(RC_ERR_UNSUPPORTED, "%s: %d x %d x %d is too large", what, M, N, K);
-  const uint32_t box[2] = {kRowBytes, BM}, box_b[2] = {kRowBytes, (uint32_t)(pair ? bn / 2 : bn)}, box_s[2] = {128, 4};
+  const uint32_t box_a[2] = {kRowBytes, (uint32_t)rows_a}, box_b[2] = {kRowBytes, (uint32_t)rows_b}, box_s[2] = {128, 4};
   const uint64_t da[2] = {(uint64_t)K, (uint64_t)M}, db[2] = {(uint64_t)K, (uint64_t)N};
   const uint64_t sta[1] = {(uint64_t)lda}, stb[1] = {(uint64_t)ldb}, sts[1] = {128};
   const uint64_t dsa[2] = {128, (uint64_t)lines_a}, dsb[2] = {128, (uint64_t)lines_b};
   const auto u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
   int r;
-  if ((r = rc::encode_tmap(&maps.a, u8, 2, const_cast<void*>(a), da, sta, box, CU_TENSOR_MAP_SWIZZLE_128B, what)))
+  if ((r = rc::encode_tmap(&maps.a, u8, 2, const_cast<void*>(a), da, sta, box_a, CU_TENSOR_MAP_SWIZZLE_128B, what)))
     return r;
   if ((r = rc::encode_tmap(&maps.b, u8, 2, const_cast<void*>(b), db, stb, box_b, CU_TENSOR_MAP_SWIZZLE_128B, what)))
     return r;
@@ -526,10 +1086,13 @@ int check_operands(const char* what, const void* a, long long lda, const void* s
   return RC_OK;
 }
 
-template <typename Out>
-int run_out(const Maps& maps, const Params& p, bool wide, cudaStream_t stream, const char* what) {
-  if (wide) return launch<256, 3, EPI_OUT, false, Out>(maps, p, stream, what);
-  return launch<128, 5, EPI_OUT, false, Out>(maps, p, stream, what);
+template <int EPI, typename Out>
+int run(const Maps& maps, const Params& p, const Plan& q, cudaStream_t stream, const char* what) {
+  if (q.bt == 16) return launch_rows<16, EPI, Out>(maps, p, q.split, stream, what);
+  if (q.bt == 32) return launch_rows<32, EPI, Out>(maps, p, q.split, stream, what);
+  if (q.pair) return launch<256, EPI == EPI_OUT ? 5 : 6, EPI, true, Out>(maps, p, stream, what);
+  if constexpr (EPI == EPI_OUT) return launch<128, 5, EPI, false, Out>(maps, p, stream, what);
+  else return launch<256, 4, EPI, false, Out>(maps, p, stream, what);
 }
 
 }  // namespace
@@ -549,10 +1112,10 @@ int rc_fp8_block_gemm(const uint8_t* a, long long lda, const uint8_t* a_scales, 
   if (!out || ldo < N || (residual && ldr < N) || reinterpret_cast<uintptr_t>(out) % 2 ||
       reinterpret_cast<uintptr_t>(residual) % 2)
     return rc::set_error(RC_ERR_ARG, "%s: out and residual must be rows of at least N columns", what);
-  const bool wide = false;
+  const Plan q = plan_for(M, N, K, false);
   Params p{};
   Maps maps;
-  if ((r = prepare(what, a, lda, a_scales, b, ldb, b_scales, M, N, K, wide ? 256 : 128, false, p, maps))) return r;
+  if ((r = prepare(what, a, lda, a_scales, b, ldb, b_scales, M, N, K, false, q, p, maps))) return r;
   p.bias = bias;
   p.out = out;
   p.ldo = ldo;
@@ -560,18 +1123,21 @@ int rc_fp8_block_gemm(const uint8_t* a, long long lda, const uint8_t* a_scales, 
   p.ldr = ldr;
   // TMA moves the output (and the residual) where rows start on 16 bytes.
   p.staged = aligned16(out) && ldo % 8 == 0 && aligned16(residual) && (!residual || ldr % 8 == 0);
-  if (p.staged) {
+  p.pairs = ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(residual)) % 4 | ldo % 2 | (residual ? ldr % 2 : 0)) == 0;
+  if (p.staged && !q.bt) {
     const auto type = out_dtype == fp8b::kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     const uint64_t dims[2] = {(uint64_t)N, (uint64_t)M};
-    const uint32_t box[2] = {64, 32};
+    const bool wide = q.bn == 256;                       // the warp's staging box (Smem::kBoxCols)
+    const uint32_t box[2] = {wide ? 32u : 64u, 32};
+    const auto swizzle = wide ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
     const uint64_t so[1] = {(uint64_t)ldo * 2}, sr[1] = {(uint64_t)ldr * 2};
-    if ((r = rc::encode_tmap(&maps.out, type, 2, out, dims, so, box, CU_TENSOR_MAP_SWIZZLE_128B, what))) return r;
+    if ((r = rc::encode_tmap(&maps.out, type, 2, out, dims, so, box, swizzle, what))) return r;
     if (residual && (r = rc::encode_tmap(&maps.res, type, 2, const_cast<void*>(residual), dims, sr, box,
-                                         CU_TENSOR_MAP_SWIZZLE_128B, what)))
+                                         swizzle, what)))
       return r;
   }
-  if (out_dtype == fp8b::kBF16) return run_out<__nv_bfloat16>(maps, p, wide, stream, what);
-  return run_out<__half>(maps, p, wide, stream, what);
+  if (out_dtype == fp8b::kBF16) return run<EPI_OUT, __nv_bfloat16>(maps, p, q, stream, what);
+  return run<EPI_OUT, __half>(maps, p, q, stream, what);
 }
 
 int rc_fp8_block_swiglu_gemm(const uint8_t* a, long long lda, const uint8_t* a_scales, const uint8_t* b,
@@ -584,14 +1150,22 @@ int rc_fp8_block_swiglu_gemm(const uint8_t* a, long long lda, const uint8_t* a_s
   if (r || !M) return r;
   if (!codes || !scales || !aligned16(codes) || !aligned16(scales))
     return rc::set_error(RC_ERR_ARG, "%s: codes and scales must be 16-byte aligned and not null", what);
+  const Plan q = plan_for(M, N, K, true);
   Params p{};
   Maps maps;
-  if ((r = prepare(what, a, lda, a_scales, b, ldb, b_scales, M, N, K, 256, false, p, maps))) return r;
+  if ((r = prepare(what, a, lda, a_scales, b, ldb, b_scales, M, N, K, true, q, p, maps))) return r;
   p.bias = bias;
   p.codes = codes;
   p.scales = scales;
   p.H = H;
-  return launch<256, 4, EPI_SWIGLU, false, __nv_bfloat16>(maps, p, stream, what);
+  if (!q.bt) {
+    const uint64_t dims[2] = {(uint64_t)H, (uint64_t)M}, stride[1] = {(uint64_t)H};
+    const uint32_t box[2] = {32, 32};
+    if ((r = rc::encode_tmap(&maps.out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, codes, dims, stride, box,
+                             CU_TENSOR_MAP_SWIZZLE_NONE, what)))
+      return r;
+  }
+  return run<EPI_SWIGLU, __nv_bfloat16>(maps, p, q, stream, what);
 }
 
 }  // extern "C"

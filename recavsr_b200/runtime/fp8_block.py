@@ -52,44 +52,57 @@ def dequantize(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
 
 def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
     """x as rows the kernels can read: unit column stride, 16-byte rows."""
-    if x.device.type != "cuda":
+    if not x.is_cuda:
         raise ValueError(f"{what}: the B200 kernels need CUDA tensors (got {x.device})")
     if x.dtype not in _DTYPES:
         raise ValueError(f"{what} takes float32 / bfloat16 / float16 rows (got {x.dtype}).")
     if x.dim() != 2:
         raise ValueError(f"{what} expects a 2-D matrix (got {x.dim()}-D).")
-    if x.shape[1] == 0 or x.shape[1] % 16:
-        raise ValueError(f"{what}: columns must be a positive multiple of 16 (got {x.shape[1]}).")
-    size = x.element_size()
-    if x.stride(1) != 1 or x.stride(0) < x.shape[1] or (x.stride(0) * size) % 16 or x.data_ptr() % 16:
-        x = x.clone(memory_format=torch.contiguous_format)
-    return x
+    n = x.shape[1]
+    if n == 0 or n % 16:
+        raise ValueError(f"{what}: columns must be a positive multiple of 16 (got {n}).")
+    if not x.is_contiguous() and (x.stride(1) != 1 or x.stride(0) < n or (x.stride(0) * x.element_size()) % 16):
+        return x.clone(memory_format=torch.contiguous_format)
+    return x.clone(memory_format=torch.contiguous_format) if x.data_ptr() % 16 else x
+
+
+def _row_stride(x: torch.Tensor) -> int:
+    """Row stride in elements (that of a contiguous matrix for a single row)."""
+    return x.shape[1] if x.is_contiguous() else x.stride(0)
 
 
 def _held(rows: int, cols: int, device) -> tuple[torch.Tensor, torch.Tensor]:
     return (torch.empty((rows, cols), dtype=torch.uint8, device=device),
-            torch.empty((scale_numel(rows, cols),), dtype=torch.uint8, device=device))
-
-
-def _quantize_impl(x: torch.Tensor, weight: bool) -> tuple[torch.Tensor, torch.Tensor]:
-    name = "quantize_weight" if weight else "quantize"
-    x = _rows(x, f"fp8_block.{name}")
-    m, k = x.shape
-    codes, scales = _held(m, k, x.device)
-    with torch.cuda.device(x.device):
-        _lib.call("rc_fp8_block_" + name, x.data_ptr(), _DTYPES[x.dtype], m, k, x.stride(0), codes.data_ptr(),
-                  scales.data_ptr(), _lib.stream(x.device))
-    return codes, scales
+            torch.empty(scale_numel(rows, cols), dtype=torch.uint8, device=device))
 
 
 def quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Rows [M, K] (fp32 / bf16 / fp16, K a multiple of 16) -> (codes, scales)."""
-    return _quantize_impl(x, False)
+    x = _rows(x, "fp8_block.quantize")
+    m, k = x.shape
+    codes, scales = _held(m, k, x.device)
+    _lib.call_on(x.get_device(), "rc_fp8_block_quantize", x.data_ptr(), _DTYPES[x.dtype], m, k, _row_stride(x),
+                 codes.data_ptr(), scales.data_ptr())
+    return codes, scales
 
 
 def quantize_weight(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Weight [N, K] -> (codes, scales), one scale for each 128 x 128 block."""
-    return _quantize_impl(weight, True)
+    w = _rows(weight, "fp8_block.quantize_weight")
+    n, k = w.shape
+    codes, scales = _held(n, k, w.device)
+    _lib.call_on(w.get_device(), "rc_fp8_block_quantize_weight", w.data_ptr(), _DTYPES[w.dtype], n, k, _row_stride(w),
+                 codes.data_ptr(), scales.data_ptr())
+    return codes, scales
+
+
+def _vector(t: torch.Tensor, n: int, like: torch.Tensor, what: str) -> torch.Tensor:
+    """A per-column vector (norm weight, bias) as 16-byte aligned fp32."""
+    if t.shape != (n,) or t.get_device() != like.get_device():
+        raise ValueError(f"{what} must have {n} elements on {like.device} (got {tuple(t.shape)} on {t.device}).")
+    if t.dtype != torch.float32 or not t.is_contiguous():
+        t = t.to(torch.float32).contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
 
 
 def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: torch.Tensor | None = None,
@@ -99,31 +112,25 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float, residua
     h = x + residual is summed in fp32; hidden is h rounded to x's dtype (None
     without a residual) and the norm h * rsqrt(mean(h^2) + eps) * weight is
     quantized from fp32, without a rounding between."""
-    what = "fp8_block.rms_norm_quantize"
-    x = _rows(x, what)
+    x = _rows(x, "fp8_block.rms_norm_quantize")
     m, n = x.shape
-    if weight.shape != (n,) or weight.device != x.device:
-        raise ValueError(f"{what}: weight must have {n} elements on {x.device}.")
+    weight = _vector(weight, n, x, "fp8_block.rms_norm_quantize: weight")
     hidden, ldr = None, 0
     if residual is not None:
-        if residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device:
-            raise ValueError(f"{what}: residual must match x's shape, dtype and device.")
-        residual = _rows(residual, what)
-        ldr = residual.stride(0)
+        if residual.shape != x.shape or residual.dtype != x.dtype or residual.get_device() != x.get_device():
+            raise ValueError("fp8_block.rms_norm_quantize: residual must match x's shape, dtype and device.")
+        residual = _rows(residual, "fp8_block.rms_norm_quantize")
+        ldr = _row_stride(residual)
         hidden = torch.empty((m, n), dtype=x.dtype, device=x.device)
-    weight = weight.to(torch.float32).contiguous()
-    if weight.data_ptr() % 16:
-        weight = weight.clone()
     codes, scales = _held(m, n, x.device)
-    with torch.cuda.device(x.device):
-        _lib.call("rc_fp8_block_rms_norm", x.data_ptr(), x.stride(0), _lib.ptr(residual), ldr, _DTYPES[x.dtype], m, n,
-                  weight.data_ptr(), float(eps), _lib.ptr(hidden), codes.data_ptr(), scales.data_ptr(),
-                  _lib.stream(x.device))
+    _lib.call_on(x.get_device(), "rc_fp8_block_rms_norm", x.data_ptr(), _row_stride(x), _lib.ptr(residual), ldr,
+                 _DTYPES[x.dtype], m, n, weight.data_ptr(), eps, _lib.ptr(hidden), codes.data_ptr(),
+                 scales.data_ptr())
     return codes, scales, hidden
 
 
 def _operand(codes: torch.Tensor, scales: torch.Tensor, what: str) -> torch.Tensor:
-    if codes.device.type != "cuda" or scales.device != codes.device:
+    if not codes.is_cuda or scales.get_device() != codes.get_device():
         raise ValueError(f"{what}: codes and scales must be on one CUDA device (got {codes.device}, {scales.device}).")
     if codes.dim() != 2 or codes.element_size() != 1 or scales.element_size() != 1:
         raise ValueError(f"{what}: operands are 8-bit codes [rows, K] with 8-bit scales.")
@@ -131,19 +138,11 @@ def _operand(codes: torch.Tensor, scales: torch.Tensor, what: str) -> torch.Tens
     if k == 0 or k % 16:
         raise ValueError(f"{what}: K must be a positive multiple of 16 (got {k}).")
     if scales.numel() != scale_numel(rows, k) or not scales.is_contiguous() or scales.data_ptr() % 16:
-        raise ValueError(f"{what}: a {rows} x {k} operand has {scale_numel(rows, k)} contiguous scale bytes.")
-    if codes.stride(1) != 1 or codes.stride(0) < k or codes.stride(0) % 16 or codes.data_ptr() % 16:
-        codes = codes.clone(memory_format=torch.contiguous_format)
-    return codes
-
-
-def _bias(bias: torch.Tensor | None, n: int, device, what: str) -> torch.Tensor | None:
-    if bias is None:
-        return None
-    if bias.shape != (n,) or bias.device != device:
-        raise ValueError(f"{what}: bias must have {n} elements on {device}.")
-    bias = bias.to(torch.float32).contiguous()
-    return bias.clone() if bias.data_ptr() % 16 else bias
+        raise ValueError(f"{what}: a {rows} x {k} operand has {scale_numel(rows, k)} contiguous, 16-byte aligned "
+                         "scale bytes.")
+    if not codes.is_contiguous() and (codes.stride(1) != 1 or codes.stride(0) < k or codes.stride(0) % 16):
+        return codes.clone(memory_format=torch.contiguous_format)
+    return codes.clone(memory_format=torch.contiguous_format) if codes.data_ptr() % 16 else codes
 
 
 def mm(values: torch.Tensor, weights: torch.Tensor, scales: torch.Tensor, weight_scales: torch.Tensor,
@@ -152,30 +151,31 @@ def mm(values: torch.Tensor, weights: torch.Tensor, scales: torch.Tensor, weight
     """[M, N] = A [M, K] . W [N, K]^T + bias (+ residual), summed in fp32 and
     rounded once to dtype (bfloat16 by default, or float16). `out` may be
     `residual` itself."""
-    what = "fp8_block.mm"
-    values, weights = _operand(values, scales, what), _operand(weights, weight_scales, what)
-    (m, k), n, dev = values.shape, weights.shape[0], values.device
-    if weights.shape[1] != k or weights.device != dev or n == 0:
-        raise ValueError(f"{what}: operands of {m} x {k} on {dev} and {n} x {weights.shape[1]} on {weights.device}.")
+    values, weights = _operand(values, scales, "fp8_block.mm"), _operand(weights, weight_scales, "fp8_block.mm")
+    (m, k), (n, kw), index = values.shape, weights.shape, values.get_device()
+    if kw != k or weights.get_device() != index or n == 0:
+        raise ValueError(f"fp8_block.mm: operands of {m} x {k} on {values.device} and {n} x {kw} on {weights.device}.")
     if dtype is None:
         dtype = out.dtype if out is not None else residual.dtype if residual is not None else torch.bfloat16
     if dtype not in _OUT:
-        raise ValueError(f"{what} produces bfloat16 or float16 (got {dtype}).")
-    bias = _bias(bias, n, dev, what)
+        raise ValueError(f"fp8_block.mm produces bfloat16 or float16 (got {dtype}).")
+    if bias is not None:
+        bias = _vector(bias, n, values, "fp8_block.mm: bias")
+    ldr = 0
     if residual is not None:
-        if residual.shape != (m, n) or residual.dtype != dtype or residual.device != dev:
-            raise ValueError(f"{what}: residual must be {m} x {n} {dtype} on {dev}.")
-        if residual.stride(1) != 1 or residual.stride(0) < n:
+        if residual.shape != (m, n) or residual.dtype != dtype or residual.get_device() != index:
+            raise ValueError(f"fp8_block.mm: residual must be {m} x {n} {dtype} on {values.device}.")
+        if not residual.is_contiguous() and (residual.stride(1) != 1 or residual.stride(0) < n):
             residual = residual.clone(memory_format=torch.contiguous_format)
+        ldr = _row_stride(residual)
     if out is None:
-        out = torch.empty((m, n), dtype=dtype, device=dev)
-    elif out.shape != (m, n) or out.dtype != dtype or out.device != dev or out.stride(1) != 1 or out.stride(0) < n:
-        raise ValueError(f"{what}: out must be {m} x {n} {dtype} rows on {dev}.")
-    with torch.cuda.device(dev):
-        _lib.call("rc_fp8_block_gemm", values.data_ptr(), values.stride(0), scales.data_ptr(), weights.data_ptr(),
-                  weights.stride(0), weight_scales.data_ptr(), _lib.ptr(bias), m, n, k, _OUT[dtype],
-                  _lib.ptr(residual), 0 if residual is None else residual.stride(0), out.data_ptr(), out.stride(0),
-                  _lib.stream(dev))
+        out = torch.empty((m, n), dtype=dtype, device=values.device)
+    elif out.shape != (m, n) or out.dtype != dtype or out.get_device() != index or (
+            not out.is_contiguous() and (out.stride(1) != 1 or out.stride(0) < n)):
+        raise ValueError(f"fp8_block.mm: out must be {m} x {n} {dtype} rows on {values.device}.")
+    _lib.call_on(index, "rc_fp8_block_gemm", values.data_ptr(), _row_stride(values), scales.data_ptr(),
+                 weights.data_ptr(), _row_stride(weights), weight_scales.data_ptr(), _lib.ptr(bias), m, n, k,
+                 _OUT[dtype], _lib.ptr(residual), ldr, out.data_ptr(), _row_stride(out))
     return out
 
 
@@ -197,20 +197,22 @@ def swiglu_mm(values: torch.Tensor, weights: torch.Tensor, scales: torch.Tensor,
     """silu(A . Wg^T + bg) * (A . Wu^T + bu) held in 8 bits: (codes, scales) of
     [M, features]. weights and bias come in interleave_gate_up's order;
     features (a multiple of 16) defaults to half the weight's rows."""
-    what = "fp8_block.swiglu_mm"
-    values, weights = _operand(values, scales, what), _operand(weights, weight_scales, what)
-    (m, k), n, dev = values.shape, weights.shape[0], values.device
-    if weights.shape[1] != k or weights.device != dev:
-        raise ValueError(f"{what}: operands of {m} x {k} on {dev} and {n} x {weights.shape[1]} on {weights.device}.")
+    values = _operand(values, scales, "fp8_block.swiglu_mm")
+    weights = _operand(weights, weight_scales, "fp8_block.swiglu_mm")
+    (m, k), (n, kw), index = values.shape, weights.shape, values.get_device()
+    if kw != k or weights.get_device() != index:
+        raise ValueError(f"fp8_block.swiglu_mm: operands of {m} x {k} on {values.device} and {n} x {kw} on "
+                         f"{weights.device}.")
     h = n // 2 if features is None else features
     if h <= 0 or h % 16 or -(-h // BLOCK) * 2 * BLOCK != n:
-        raise ValueError(f"{what}: {h} features need {-(-h // BLOCK) * 2 * BLOCK} interleaved weight rows (got {n}).")
-    bias = _bias(bias, n, dev, what)
-    codes, out_scales = _held(m, h, dev)
-    with torch.cuda.device(dev):
-        _lib.call("rc_fp8_block_swiglu_gemm", values.data_ptr(), values.stride(0), scales.data_ptr(),
-                  weights.data_ptr(), weights.stride(0), weight_scales.data_ptr(), _lib.ptr(bias), m, h, k,
-                  codes.data_ptr(), out_scales.data_ptr(), _lib.stream(dev))
+        raise ValueError(f"fp8_block.swiglu_mm: {h} features need {-(-h // BLOCK) * 2 * BLOCK} interleaved weight "
+                         f"rows (got {n}).")
+    if bias is not None:
+        bias = _vector(bias, n, values, "fp8_block.swiglu_mm: bias")
+    codes, out_scales = _held(m, h, values.device)
+    _lib.call_on(index, "rc_fp8_block_swiglu_gemm", values.data_ptr(), _row_stride(values), scales.data_ptr(),
+                 weights.data_ptr(), _row_stride(weights), weight_scales.data_ptr(), _lib.ptr(bias), m, h, k,
+                 codes.data_ptr(), out_scales.data_ptr())
     return codes, out_scales
 
 
