@@ -132,21 +132,6 @@ def stream(device: torch.device | None = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def call_on(index: int, name: str, *args) -> None:
-    """call(name, *args, stream) on the current stream of CUDA device `index`,
-    with that device current: the short way for calls of a few microseconds
-    (the raw stream handle instead of a Stream object, and no device switch
-    where the device is current already)."""
-    fn = getattr(_lib or library(), name)
-    if torch.cuda.current_device() == index:
-        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(index):
-            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    if status:
-        check(status, name)
-
-
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 

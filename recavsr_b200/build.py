@@ -3,7 +3,9 @@
     python -m recavsr_b200.build          # incremental
     python -m recavsr_b200.build --force  # rebuild everything
 
-Objects go to recavsr_b200/_build/, the library to recavsr_b200/librecavsr_b200.so.
+Objects go to recavsr_b200/_build/, the library to recavsr_b200/librecavsr_b200.so
+and the Python binding of the block-scaled FP8 operators (a CPython extension on
+torch's C++ headers, linked to the library) to recavsr_b200/_fp8_block.so.
 The CUDA runtime is linked statically; the driver is reached through
 cudaGetDriverEntryPoint, so the library needs no -lcuda at link time.
 """
@@ -14,11 +16,15 @@ import concurrent.futures as cf
 import os
 import shutil
 import subprocess
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 OBJ = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "librecavsr_b200.so")
+BINDING = os.path.join(PKG, "_fp8_block.so")
+BINDING_SOURCE = os.path.join(CSRC, "fp8_block_torch.cpp")
+INCLUDE = os.path.join(os.path.dirname(PKG), "include", "recavsr_b200.h")
 SOURCES = ["runtime.cu", "quant.cu", "glue.cu", "gemm.cu", "attention.cu", "session.cu", "pipeline.cu", "decoder_attention.cu", "decoder.cu", "colorfix.cu",
            "fp8_block.cu", "fp8_block_gemm.cu"]
 HEADERS = ["common.cuh", "sm100.cuh", "fp8_block.cuh"]
@@ -52,6 +58,26 @@ def _compile(src: str, force: bool) -> str:
     return obj
 
 
+def _build_binding(force: bool) -> None:
+    if not force and not _stale(BINDING, [BINDING_SOURCE, INCLUDE]):
+        return
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc()))), "include")
+    include = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+               sysconfig.get_paths()["include"], cuda]
+    # The host compiler that nvcc uses, not $CXX: one with a C++ runtime of its
+    # own linked in clashes with the runtime torch has loaded.
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{d}" for d in include),
+           BINDING_SOURCE, "-o", BINDING, "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10",
+           "-lc10_cuda", "-L" + PKG, "-l:" + os.path.basename(LIB), "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode:
+        raise RuntimeError(f"{cmd[0]} failed for {os.path.basename(BINDING_SOURCE)}:\n{r.stderr}")
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(OBJ, exist_ok=True)
     with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
@@ -61,6 +87,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode:
             raise RuntimeError(f"link failed:\n{r.stderr}")
+    _build_binding(force)
     if verbose:
         print(LIB)
     return LIB

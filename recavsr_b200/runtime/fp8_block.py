@@ -22,11 +22,13 @@ from __future__ import annotations
 import torch
 from torch import nn
 
-from .. import _lib
+try:
+    from .. import _fp8_block as _binding
+except ImportError as error:
+    raise ImportError("recavsr_b200/_fp8_block.so cannot be loaded: build it with `python -m recavsr_b200.build` "
+                      "(there is no CPU fallback)") from error
 
 BLOCK = 128
-_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_OUT = {torch.bfloat16: 1, torch.float16: 2}
 
 
 def scale_numel(rows: int, cols: int) -> int:
@@ -50,59 +52,18 @@ def dequantize(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
     return values * power.repeat_interleave(BLOCK, 1)[:, :cols]
 
 
-def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
-    """x as rows the kernels can read: unit column stride, 16-byte rows."""
-    if not x.is_cuda:
-        raise ValueError(f"{what}: the B200 kernels need CUDA tensors (got {x.device})")
-    if x.dtype not in _DTYPES:
-        raise ValueError(f"{what} takes float32 / bfloat16 / float16 rows (got {x.dtype}).")
-    if x.dim() != 2:
-        raise ValueError(f"{what} expects a 2-D matrix (got {x.dim()}-D).")
-    n = x.shape[1]
-    if n == 0 or n % 16:
-        raise ValueError(f"{what}: columns must be a positive multiple of 16 (got {n}).")
-    if not x.is_contiguous() and (x.stride(1) != 1 or x.stride(0) < n or (x.stride(0) * x.element_size()) % 16):
-        return x.clone(memory_format=torch.contiguous_format)
-    return x.clone(memory_format=torch.contiguous_format) if x.data_ptr() % 16 else x
-
-
-def _row_stride(x: torch.Tensor) -> int:
-    """Row stride in elements (that of a contiguous matrix for a single row)."""
-    return x.shape[1] if x.is_contiguous() else x.stride(0)
-
-
-def _held(rows: int, cols: int, device) -> tuple[torch.Tensor, torch.Tensor]:
-    return (torch.empty((rows, cols), dtype=torch.uint8, device=device),
-            torch.empty(scale_numel(rows, cols), dtype=torch.uint8, device=device))
-
-
 def quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Rows [M, K] (fp32 / bf16 / fp16, K a multiple of 16) -> (codes, scales)."""
-    x = _rows(x, "fp8_block.quantize")
-    m, k = x.shape
-    codes, scales = _held(m, k, x.device)
-    _lib.call_on(x.get_device(), "rc_fp8_block_quantize", x.data_ptr(), _DTYPES[x.dtype], m, k, _row_stride(x),
-                 codes.data_ptr(), scales.data_ptr())
-    return codes, scales
+    if torch.compiler.is_compiling():
+        return torch.ops.recavsr_b200.fp8_block_quantize(x, False)
+    return _binding.quantize(x, False)
 
 
 def quantize_weight(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Weight [N, K] -> (codes, scales), one scale for each 128 x 128 block."""
-    w = _rows(weight, "fp8_block.quantize_weight")
-    n, k = w.shape
-    codes, scales = _held(n, k, w.device)
-    _lib.call_on(w.get_device(), "rc_fp8_block_quantize_weight", w.data_ptr(), _DTYPES[w.dtype], n, k, _row_stride(w),
-                 codes.data_ptr(), scales.data_ptr())
-    return codes, scales
-
-
-def _vector(t: torch.Tensor, n: int, like: torch.Tensor, what: str) -> torch.Tensor:
-    """A per-column vector (norm weight, bias) as 16-byte aligned fp32."""
-    if t.shape != (n,) or t.get_device() != like.get_device():
-        raise ValueError(f"{what} must have {n} elements on {like.device} (got {tuple(t.shape)} on {t.device}).")
-    if t.dtype != torch.float32 or not t.is_contiguous():
-        t = t.to(torch.float32).contiguous()
-    return t.clone() if t.data_ptr() % 16 else t
+    if torch.compiler.is_compiling():
+        return torch.ops.recavsr_b200.fp8_block_quantize(weight, True)
+    return _binding.quantize(weight, True)
 
 
 def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: torch.Tensor | None = None,
@@ -111,72 +72,20 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float, residua
 
     h = x + residual is summed in fp32; hidden is h rounded to x's dtype (None
     without a residual) and the norm h * rsqrt(mean(h^2) + eps) * weight is
-    quantized from fp32, without a rounding between."""
-    x = _rows(x, "fp8_block.rms_norm_quantize")
-    m, n = x.shape
-    weight = _vector(weight, n, x, "fp8_block.rms_norm_quantize: weight")
-    hidden, ldr = None, 0
-    if residual is not None:
-        if residual.shape != x.shape or residual.dtype != x.dtype or residual.get_device() != x.get_device():
-            raise ValueError("fp8_block.rms_norm_quantize: residual must match x's shape, dtype and device.")
-        residual = _rows(residual, "fp8_block.rms_norm_quantize")
-        ldr = _row_stride(residual)
-        hidden = torch.empty((m, n), dtype=x.dtype, device=x.device)
-    codes, scales = _held(m, n, x.device)
-    _lib.call_on(x.get_device(), "rc_fp8_block_rms_norm", x.data_ptr(), _row_stride(x), _lib.ptr(residual), ldr,
-                 _DTYPES[x.dtype], m, n, weight.data_ptr(), eps, _lib.ptr(hidden), codes.data_ptr(),
-                 scales.data_ptr())
-    return codes, scales, hidden
-
-
-def _operand(codes: torch.Tensor, scales: torch.Tensor, what: str) -> torch.Tensor:
-    if not codes.is_cuda or scales.get_device() != codes.get_device():
-        raise ValueError(f"{what}: codes and scales must be on one CUDA device (got {codes.device}, {scales.device}).")
-    if codes.dim() != 2 or codes.element_size() != 1 or scales.element_size() != 1:
-        raise ValueError(f"{what}: operands are 8-bit codes [rows, K] with 8-bit scales.")
-    rows, k = codes.shape
-    if k == 0 or k % 16:
-        raise ValueError(f"{what}: K must be a positive multiple of 16 (got {k}).")
-    if scales.numel() != scale_numel(rows, k) or not scales.is_contiguous() or scales.data_ptr() % 16:
-        raise ValueError(f"{what}: a {rows} x {k} operand has {scale_numel(rows, k)} contiguous, 16-byte aligned "
-                         "scale bytes.")
-    if not codes.is_contiguous() and (codes.stride(1) != 1 or codes.stride(0) < k or codes.stride(0) % 16):
-        return codes.clone(memory_format=torch.contiguous_format)
-    return codes.clone(memory_format=torch.contiguous_format) if codes.data_ptr() % 16 else codes
+    quantized from fp32, without a rounding between. Rows of at most 16384
+    columns, a multiple of 16."""
+    return _binding.rms_norm_quantize(x, weight, eps, residual)
 
 
 def mm(values: torch.Tensor, weights: torch.Tensor, scales: torch.Tensor, weight_scales: torch.Tensor,
        bias: torch.Tensor | None = None, *, residual: torch.Tensor | None = None,
        dtype: torch.dtype | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """[M, N] = A [M, K] . W [N, K]^T + bias (+ residual), summed in fp32 and
-    rounded once to dtype (bfloat16 by default, or float16). `out` may be
-    `residual` itself."""
-    values, weights = _operand(values, scales, "fp8_block.mm"), _operand(weights, weight_scales, "fp8_block.mm")
-    (m, k), (n, kw), index = values.shape, weights.shape, values.get_device()
-    if kw != k or weights.get_device() != index or n == 0:
-        raise ValueError(f"fp8_block.mm: operands of {m} x {k} on {values.device} and {n} x {kw} on {weights.device}.")
-    if dtype is None:
-        dtype = out.dtype if out is not None else residual.dtype if residual is not None else torch.bfloat16
-    if dtype not in _OUT:
-        raise ValueError(f"fp8_block.mm produces bfloat16 or float16 (got {dtype}).")
-    if bias is not None:
-        bias = _vector(bias, n, values, "fp8_block.mm: bias")
-    ldr = 0
-    if residual is not None:
-        if residual.shape != (m, n) or residual.dtype != dtype or residual.get_device() != index:
-            raise ValueError(f"fp8_block.mm: residual must be {m} x {n} {dtype} on {values.device}.")
-        if not residual.is_contiguous() and (residual.stride(1) != 1 or residual.stride(0) < n):
-            residual = residual.clone(memory_format=torch.contiguous_format)
-        ldr = _row_stride(residual)
-    if out is None:
-        out = torch.empty((m, n), dtype=dtype, device=values.device)
-    elif out.shape != (m, n) or out.dtype != dtype or out.get_device() != index or (
-            not out.is_contiguous() and (out.stride(1) != 1 or out.stride(0) < n)):
-        raise ValueError(f"fp8_block.mm: out must be {m} x {n} {dtype} rows on {values.device}.")
-    _lib.call_on(index, "rc_fp8_block_gemm", values.data_ptr(), _row_stride(values), scales.data_ptr(),
-                 weights.data_ptr(), _row_stride(weights), weight_scales.data_ptr(), _lib.ptr(bias), m, n, k,
-                 _OUT[dtype], _lib.ptr(residual), ldr, out.data_ptr(), _row_stride(out))
-    return out
+    rounded once to dtype (bfloat16 by default, or float16; the residual has the
+    same). `out` may be `residual` itself."""
+    if torch.compiler.is_compiling() and out is None:
+        return torch.ops.recavsr_b200.fp8_block_mm(values, weights, scales, weight_scales, bias, residual, dtype)
+    return _binding.mm(values, weights, scales, weight_scales, bias, residual, dtype, out)
 
 
 def interleave_gate_up(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
@@ -197,23 +106,30 @@ def swiglu_mm(values: torch.Tensor, weights: torch.Tensor, scales: torch.Tensor,
     """silu(A . Wg^T + bg) * (A . Wu^T + bu) held in 8 bits: (codes, scales) of
     [M, features]. weights and bias come in interleave_gate_up's order;
     features (a multiple of 16) defaults to half the weight's rows."""
-    values = _operand(values, scales, "fp8_block.swiglu_mm")
-    weights = _operand(weights, weight_scales, "fp8_block.swiglu_mm")
-    (m, k), (n, kw), index = values.shape, weights.shape, values.get_device()
-    if kw != k or weights.get_device() != index:
-        raise ValueError(f"fp8_block.swiglu_mm: operands of {m} x {k} on {values.device} and {n} x {kw} on "
-                         f"{weights.device}.")
-    h = n // 2 if features is None else features
-    if h <= 0 or h % 16 or -(-h // BLOCK) * 2 * BLOCK != n:
-        raise ValueError(f"fp8_block.swiglu_mm: {h} features need {-(-h // BLOCK) * 2 * BLOCK} interleaved weight "
-                         f"rows (got {n}).")
-    if bias is not None:
-        bias = _vector(bias, n, values, "fp8_block.swiglu_mm: bias")
-    codes, out_scales = _held(m, h, values.device)
-    _lib.call_on(index, "rc_fp8_block_swiglu_gemm", values.data_ptr(), _row_stride(values), scales.data_ptr(),
-                 weights.data_ptr(), _row_stride(weights), weight_scales.data_ptr(), _lib.ptr(bias), m, h, k,
-                 codes.data_ptr(), out_scales.data_ptr())
-    return codes, out_scales
+    return _binding.swiglu_mm(values, weights, scales, weight_scales, bias, features)
+
+
+@torch.library.custom_op("recavsr_b200::fp8_block_quantize", mutates_args=())
+def _quantize_op(x: torch.Tensor, weight: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    return _binding.quantize(x, weight)
+
+
+@_quantize_op.register_fake
+def _quantize_fake(x, weight):
+    return (x.new_empty(x.shape, dtype=torch.uint8),
+            x.new_empty((scale_numel(*x.shape),), dtype=torch.uint8))
+
+
+@torch.library.custom_op("recavsr_b200::fp8_block_mm", mutates_args=())
+def _mm_op(values: torch.Tensor, weights: torch.Tensor, scales: torch.Tensor, weight_scales: torch.Tensor,
+           bias: torch.Tensor | None, residual: torch.Tensor | None, dtype: torch.dtype | None) -> torch.Tensor:
+    return _binding.mm(values, weights, scales, weight_scales, bias, residual, dtype, None)
+
+
+@_mm_op.register_fake
+def _mm_fake(values, weights, scales, weight_scales, bias, residual, dtype):
+    dtype = dtype or (torch.bfloat16 if residual is None else residual.dtype)
+    return values.new_empty((values.shape[0], weights.shape[0]), dtype=dtype)
 
 
 class BlockFP8Linear(nn.Module):
@@ -234,7 +150,7 @@ class BlockFP8Linear(nn.Module):
         self.register_buffer("bias", None if linear.bias is None else linear.bias.detach().float())
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        if x.dtype not in _OUT:
+        if x.dtype not in (torch.bfloat16, torch.float16):
             raise ValueError("Block FP8 linears take BF16 or FP16 inputs and produce the same type.")
         codes, scales = quantize(x.reshape(-1, self.in_features))
         out = mm(codes, self.weight_codes, scales, self.weight_scales, self.bias, dtype=x.dtype)

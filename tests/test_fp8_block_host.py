@@ -75,6 +75,11 @@ def test_cpu_tensors_are_refused():
                  lambda: fp8_block.swiglu_mm(codes, codes, scales, scales)):
         with pytest.raises(ValueError, match="CUDA"):
             call()
+    from recavsr_b200 import _fp8_block
+    with pytest.raises(RuntimeError, match="expected 8 arguments"):
+        _fp8_block.mm(codes, codes, scales, scales)
+    with pytest.raises(ValueError, match="tensor"):
+        fp8_block.quantize("x")
 
 
 def test_entry_points_reject_bad_arguments():

@@ -421,6 +421,20 @@ def test_linear():
     assert isinstance(model[0], fp8_block.BlockFP8Linear)
 
 
+def test_linear_compiles():
+    """torch.compile(fullgraph=True) traces through BlockFP8Linear."""
+    from recavsr_b200.runtime import fp8_block
+    torch.manual_seed(0)
+    model = torch.nn.Sequential(torch.nn.Linear(256, 512), torch.nn.GELU(), torch.nn.Linear(512, 128))
+    model = model.to("cuda", torch.bfloat16)
+    fp8_block.quantize_block_linears(model)
+    x = activations(37, 256, torch.bfloat16, 24)
+    with torch.inference_mode():
+        want = model(x)
+        got = torch.compile(model, fullgraph=True, backend="aot_eager")(x)
+    assert torch.equal(got, want)
+
+
 def test_refusals():
     from recavsr_b200.runtime import fp8_block
     x = torch.zeros(4, 64, dtype=torch.bfloat16, device="cuda")
