@@ -19,6 +19,12 @@ rc_local_gqa_attention -> output GEMM (+ residual) -> RMSNorm -> fused
 gate|up GEMM with the SwiGLU epilogue -> down GEMM (+ residual): nine launches, all of
 this library's kernels. Steady-state steps are replayed from CUDA graphs
 (capture(): one per parity of the ring positions, which repeat every two steps).
+
+With linears="fp8_block" the blocks' linears run on block-scaled FP8 operands
+(runtime.fp8_block): the norms produce their rows in 8 bits, the attention
+output is quantized for its projection and the gated product leaves its
+activations in 8 bits; what a projection adds to the residual stream is added by
+the norm that follows it. The reference's decoder has no 8-bit form.
 """
 from __future__ import annotations
 
@@ -82,6 +88,9 @@ class _Stack:
             pre = f"{prefix}.blocks.{i}."
             a = pre + "attention."
             w = d.params
+            if d.fp8:
+                self.layers.append(self._fp8_layer(d, pre, ring_tokens))
+                continue
             self.layers.append(dict(
                 attn_w=_dev(w[pre + "attention_norm.weight"], dev, torch.float32),
                 ffn_w=_dev(w[pre + "feed_forward_norm.weight"], dev, torch.float32),
@@ -102,6 +111,25 @@ class _Stack:
                 v_ring=torch.zeros((d.hk, ring_tokens, HEAD_DIM), dtype=torch.bfloat16, device=dev)))
         self.ring_head = ring_tokens * HEAD_DIM
 
+    @staticmethod
+    def _fp8_layer(d, pre, ring_tokens):
+        """A block's parameters with its linears held in block-scaled FP8."""
+        from . import fp8_block
+        w, dev, a, f = d.params, d.device, pre + "attention.", pre + "feed_forward."
+        fp32 = lambda name: _dev(w[name], dev, torch.float32)
+        qkv = [a + x for x in ("query", "key", "value")]
+        gate_up = lambda part: fp8_block.interleave_gate_up(fp32(f + "gate" + part), fp32(f + "up" + part))
+        return dict(
+            attn_w=fp32(pre + "attention_norm.weight"), ffn_w=fp32(pre + "feed_forward_norm.weight"),
+            qkv_w=fp8_block.quantize_weight(torch.cat([fp32(x + ".weight") for x in qkv])),
+            qkv_b=torch.cat([fp32(x + ".bias") for x in qkv]),
+            kn=fp32(a + "key_norm.weight"), vn=fp32(a + "value_norm.weight"),
+            o_w=fp8_block.quantize_weight(fp32(a + "output.weight")), o_b=fp32(a + "output.bias"),
+            gu_w=fp8_block.quantize_weight(gate_up(".weight")), gu_b=gate_up(".bias"),
+            d_w=fp8_block.quantize_weight(fp32(f + "down.weight")), d_b=fp32(f + "down.bias"),
+            k_ring=torch.zeros((d.hk, ring_tokens, HEAD_DIM), dtype=torch.float32, device=dev),
+            v_ring=torch.zeros((d.hk, ring_tokens, HEAD_DIM), dtype=torch.bfloat16, device=dev))
+
     def positions(self):
         """(prev, nf, slot0, slot_w) of the next step: the trimmed cache keeps
         the last max_frames - cur frames written (flashdecoder_wan22.py:428-437),
@@ -117,11 +145,15 @@ class DecoderSession:
 
     params: the FlashDecoder state dict (tensors or arrays, reference names);
     mean / std: the 48 latent normalization values (vae_config latents_mean /
-    latents_std); height / width: the latent grid (output 16x that)."""
+    latents_std); height / width: the latent grid (output 16x that); linears:
+    "bf16", or "fp8_block" for block-scaled FP8 linears in the blocks."""
 
     def __init__(self, params, *, height, width, mean, std, dim=512, num_heads=8, num_kv_groups=2, depth=12,
                  refinement_depth=2, mlp_ratio=4.0, window=(24, 24), window_size=2, eps=1e-5,
-                 rope_theta=10000.0, device=None):
+                 rope_theta=10000.0, device=None, linears="bf16"):
+        if linears not in ("bf16", "fp8_block"):
+            raise ValueError(f'linears must be "bf16" or "fp8_block" (got {linears!r}).')
+        self.fp8 = linears == "fp8_block"
         from .flashdecoder import validate_spatial_window
         self.window = validate_spatial_window(tuple(window))
         if dim % num_heads or num_heads % num_kv_groups or dim // num_heads != HEAD_DIM:
@@ -163,6 +195,12 @@ class DecoderSession:
         self.x, self.hr, self.xn = e(n, dim), e(t4, dim), e(t4, dim)
         self.qkv, self.q_rot, self.att = e(t4, qkv_n), e(t4, dim), e(t4, dim)
         self.act = e(t4, self.hidden)
+        if self.fp8:
+            from .fp8_block import scale_numel
+            u8 = torch.uint8
+            self.rows8, self.rows8_s = e(t4, dim, dt=u8), e(scale_numel(t4, dim), dt=u8)
+            self.act8, self.act8_s = e(t4, self.hidden, dt=u8), e(scale_numel(t4, self.hidden), dt=u8)
+            self.delta = e(t4, dim)
         self.s2 = e(t4, 768)
         self.lat_in, self.unsh, self.feats = e(n, 64), e(t4, 768), e(t4, 48)
         self.grouped, self.late_in = e(n, 192), e(t4, 64)
@@ -187,6 +225,18 @@ class DecoderSession:
         _lib.call("rc_layer_norm", x.data_ptr(), 1, self.dim, rows, self.dim, weight.data_ptr(), None, self.eps, 1,
                   out.data_ptr(), self.dim, self.stream)
 
+    def _norm8(self, x, weight, rows, add):
+        """x += delta (with `add`), then RMSNorm(x) held in 8 bits in rows8."""
+        src, res = (self.delta, x) if add else (x, None)
+        _lib.call("rc_fp8_block_rms_norm", src.data_ptr(), self.dim, _lib.ptr(res), self.dim, 1, rows, self.dim,
+                  weight.data_ptr(), self.eps, _lib.ptr(res), self.rows8.data_ptr(), self.rows8_s.data_ptr(),
+                  self.stream)
+
+    def _mm8(self, a, a_scales, w, b, m, n, k, residual, out):
+        codes, scales = w
+        _lib.call("rc_fp8_block_gemm", a.data_ptr(), k, a_scales.data_ptr(), codes.data_ptr(), k, scales.data_ptr(),
+                  b.data_ptr(), m, n, k, 1, _lib.ptr(residual), n, out.data_ptr(), n, self.stream)
+
     def _stack(self, st: _Stack, x: torch.Tensor, positions):
         prev, nf, slot0, slot_w = positions
         cur, n, dim = st.cur, self.n, self.dim
@@ -196,9 +246,13 @@ class DecoderSession:
                                    self.hk * nf * n * HEAD_DIM, nf * n * HEAD_DIM, HEAD_DIM,
                                    self.hk * nf * n * HEAD_DIM, nf * n * HEAD_DIM, HEAD_DIM)
         o_str = (C.c_longlong * 3)(tokens * dim, HEAD_DIM, dim)
-        for L in st.layers:
-            self._rms(x, L["attn_w"], tokens, self.xn)
-            self._gemm(self.xn, L["qkv_w"], L["qkv_b"], tokens, qkv_n, dim, EPI_BIAS, self.qkv, qkv_n)
+        for i, L in enumerate(st.layers):
+            if self.fp8:
+                self._norm8(x, L["attn_w"], tokens, add=i > 0)
+                self._mm8(self.rows8, self.rows8_s, L["qkv_w"], L["qkv_b"], tokens, qkv_n, dim, None, self.qkv)
+            else:
+                self._rms(x, L["attn_w"], tokens, self.xn)
+                self._gemm(self.xn, L["qkv_w"], L["qkv_b"], tokens, qkv_n, dim, EPI_BIAS, self.qkv, qkv_n)
             _lib.call("rc_fd_kv_norm", self.qkv.data_ptr(), qkv_n, tokens, dim, self.hk, L["kn"].data_ptr(),
                       L["vn"].data_ptr(), self.eps, L["k_ring"].data_ptr(), L["v_ring"].data_ptr(), st.ring_head,
                       slot_w * n, self.stream)
@@ -209,6 +263,19 @@ class DecoderSession:
             _lib.call("rc_local_gqa_attention", self.q_rot.data_ptr(), self.kbuf.data_ptr(), self.vbuf.data_ptr(),
                       q_str, 1, self.hq, self.hk, cur, nf, self.h, self.w, HEAD_DIM, self.window[0],
                       self.window[1], cur, st.max_frames // cur, 0, self.att.data_ptr(), o_str, self.stream)
+            if self.fp8:
+                _lib.call("rc_fp8_block_quantize", self.att.data_ptr(), 1, tokens, dim, dim, self.rows8.data_ptr(),
+                          self.rows8_s.data_ptr(), self.stream)
+                self._mm8(self.rows8, self.rows8_s, L["o_w"], L["o_b"], tokens, dim, dim, None, self.delta)
+                self._norm8(x, L["ffn_w"], tokens, add=True)
+                codes, scales = L["gu_w"]
+                _lib.call("rc_fp8_block_swiglu_gemm", self.rows8.data_ptr(), dim, self.rows8_s.data_ptr(),
+                          codes.data_ptr(), dim, scales.data_ptr(), L["gu_b"].data_ptr(), tokens, self.hidden, dim,
+                          self.act8.data_ptr(), self.act8_s.data_ptr(), self.stream)
+                last = i + 1 == len(st.layers)      # no norm of this stack follows: the product adds
+                self._mm8(self.act8, self.act8_s, L["d_w"], L["d_b"], tokens, dim, self.hidden, x if last else None,
+                          x if last else self.delta)
+                continue
             self._gemm(self.att, L["o_w"], L["o_b"], tokens, dim, dim, EPI_RESIDUAL, x, dim)
             self._rms(x, L["ffn_w"], tokens, self.xn)
             # gate | up GEMM with the SwiGLU epilogue: act = bf16(bf16(silu(gate)) * up)
@@ -374,13 +441,14 @@ class DecoderSession:
             self._copy.synchronize()
 
     @classmethod
-    def from_module(cls, model, *, height, width, mean, std, device=None):
+    def from_module(cls, model, *, height, width, mean, std, device=None, linears="bf16"):
         """From a reference FlashDecoder module (its state dict and sizes)."""
         return cls({k: v.float() for k, v in model.state_dict().items()}, height=height, width=width, mean=mean,
                    std=std, dim=model.dim, num_heads=model.num_heads, num_kv_groups=model.num_kv_groups,
                    depth=model.depth, refinement_depth=model.refinement_depth,
                    mlp_ratio=model.backbone.blocks[0].feed_forward.gate.out_features / model.dim,
-                   window=model.spatial_window_size, window_size=model.window_size, device=device)
+                   window=model.spatial_window_size, window_size=model.window_size, device=device,
+                   linears=linears)
 
 
 def random_params(device, seed=0, *, dim=512, hidden=2048, depth=12, refinement_depth=2, kv_dim=128):
