@@ -16,7 +16,9 @@
 // One CTA per SM (or CTA pair, PAIR: 256-row tiles over two SMs, each staging
 // its own 128 rows of A and half of W's) walks the output tiles: warp 0 = TMA
 // producer, warp 1 = MMA issuer, the other warps = epilogue, 64 columns of one
-// accumulator row per thread.
+// accumulator row per thread. The accumulator is drained into registers and
+// released before the epilogue's arithmetic; tiles of 128 and 192 columns have
+// more than one accumulator, so the next tile's MMAs do not wait for that.
 #include "fp8_block.cuh"
 #include "sm100.cuh"
 
@@ -52,6 +54,9 @@ struct Maps {
 
 template <int BN>
 constexpr int epi_warps() { return BN / 16; }        // 4 lane quadrants x BN / 64 column shares
+// Scale atoms (128 rows of W) under BN columns that start on a multiple of BN.
+template <int BN>
+constexpr int sfb_atoms() { return BN % 128 ? (BN + 64) / 128 : BN / 128; }
 template <int BN>
 constexpr int tile_threads() { return 64 + 32 * epi_warps<BN>(); }
 
@@ -59,7 +64,7 @@ template <int BN, int STAGES, int EPI, bool PAIR>
 struct Smem {
   static constexpr int kA = BM * kRowBytes;
   static constexpr int kB = (PAIR ? BN / 2 : BN) * kRowBytes;    // a pair splits W's rows between its CTAs
-  static constexpr int kSf = (1 + BN / 128) * kSfAtom;
+  static constexpr int kSf = (1 + sfb_atoms<BN>()) * kSfAtom;
   static constexpr int offA = 0;
   static constexpr int offB = offA + STAGES * kA;
   static constexpr int offOut = offB + STAGES * kB;
@@ -189,8 +194,9 @@ __global__ void __launch_bounds__(tile_threads<BN>(), 1)
 tile_kernel(const __grid_constant__ Maps maps, const Params p) {
   using S = Smem<BN, STAGES, EPI, PAIR>;
   constexpr int kEpiWarps = epi_warps<BN>();
-  constexpr int kAcc = BN == 128 ? 3 : 1;           // accumulators in TMEM
-  constexpr int kSfaCols = 4, kSfbCols = 4 * (BN / 128), kSfCols = kSfaCols + kSfbCols;
+  constexpr int kAcc = BN == 128 ? 3 : BN == 192 ? 2 : 1;           // accumulators in TMEM
+  constexpr int kSfaCols = 4, kSfbCols = 4 * sfb_atoms<BN>(), kSfCols = kSfaCols + kSfbCols;
+  static_assert(EPI == EPI_OUT || BN == 256, "SWIGLU tiles are one block of 128 outputs");
   constexpr int kTmemCols = 512;
   static_assert(kAcc * BN + 2 * kSfCols <= kTmemCols, "TMEM budget");
 
@@ -268,7 +274,8 @@ tile_kernel(const __grid_constant__ Maps maps, const Params p) {
         int mb, nb;
         walk.coords(p, mb, nb);
         const int rb = PAIR ? mb * 2 + (int)rank : mb;                          // this CTA's 128-row block of A
-        const int brow = PAIR ? nb * BN + (int)rank * (BN / 2) : nb * BN;       // and its first row of W
+        const int brow = nb * BN + (PAIR ? (int)rank * (BN / 2) : 0);    // and its first row of W
+        const int b_line = nb * BN / 128 * p.katoms * 4;
         for (int kt = 0; kt < p.k_tiles; ++kt) {
           if (!wait(&empty[stage], phase ^ 1, 1)) { ok = false; break; }
           uint8_t* a = smem + S::offA + stage * S::kA;
@@ -284,9 +291,8 @@ tile_kernel(const __grid_constant__ Maps maps, const Params p) {
             sm100::tma_load_2d_pair(b, &maps.b, bar, kt * kRowBytes, brow);
             if (atom) {
               sm100::tma_load_2d_pair(sf, &maps.sfa, bar, 0, rb * p.katoms * 4 + line);
-              for (int r = 0; r < BN / 128; ++r)
-                sm100::tma_load_2d_pair(sf + (1 + r) * kSfAtom, &maps.sfb, bar, 0,
-                                        (nb * (BN / 128) + r) * p.katoms * 4 + line);
+              for (int r = 0; r < sfb_atoms<BN>(); ++r)
+                sm100::tma_load_2d_pair(sf + (1 + r) * kSfAtom, &maps.sfb, bar, 0, b_line + r * p.katoms * 4 + line);
             }
           } else {
             sm100::mbar_arrive_expect_tx(&full[stage], bytes);
@@ -294,9 +300,8 @@ tile_kernel(const __grid_constant__ Maps maps, const Params p) {
             sm100::tma_load_2d(b, &maps.b, &full[stage], kt * kRowBytes, brow);
             if (atom) {
               sm100::tma_load_2d(sf, &maps.sfa, &full[stage], 0, rb * p.katoms * 4 + line);
-              for (int r = 0; r < BN / 128; ++r)
-                sm100::tma_load_2d(sf + (1 + r) * kSfAtom, &maps.sfb, &full[stage], 0,
-                                   (nb * (BN / 128) + r) * p.katoms * 4 + line);
+              for (int r = 0; r < sfb_atoms<BN>(); ++r)
+                sm100::tma_load_2d(sf + (1 + r) * kSfAtom, &maps.sfb, &full[stage], 0, b_line + r * p.katoms * 4 + line);
             }
           }
           ++issued;
@@ -326,7 +331,17 @@ tile_kernel(const __grid_constant__ Maps maps, const Params p) {
         if constexpr (PAIR) sm100::tc_commit_pair(bar);   // arrives in both CTAs
         else sm100::tc_commit(bar);
       };
+      Walk walk(p, tile0);
       for (int tile = tile0; tile < tiles && ok; tile += step, ++local) {
+        // The scale rows of a tile that starts in the middle of an atom begin
+        // two columns (64 rows) into its copy.
+        uint32_t shift = 0;
+        if constexpr (BN % 128 != 0) {
+          int mb, nb;
+          walk.coords(p, mb, nb);
+          shift = (uint32_t)(nb & 1) * 2;
+          walk.next(p, step);
+        }
         const int as = local % kAcc;
         if (!wait(&acc_empty[as], (uint32_t)((local / kAcc) & 1) ^ 1, 2)) { ok = false; break; }
         sm100::tc_fence_after();
@@ -343,19 +358,19 @@ tile_kernel(const __grid_constant__ Maps maps, const Params p) {
             sfb = sfa + kSfaCols;
             const uint64_t dsf = sm100::desc_add(dsf0, stage * S::kSf);
 #pragma unroll
-            for (int r = 0; r < 1 + BN / 128; ++r) {
+            for (int r = 0; r < 1 + sfb_atoms<BN>(); ++r) {
               if constexpr (PAIR) sm100::tmem_cp_32x128b_warpx4_pair(sfa + 4 * r, sm100::desc_add(dsf, r * kSfAtom));
               else sm100::tmem_cp_32x128b_warpx4(sfa + 4 * r, sm100::desc_add(dsf, r * kSfAtom));
             }
           }
           const uint32_t idesc = sm100::idesc_mxf8(PAIR ? 2 * BM : BM, BN, 0) | ((kt & 3) << 4) | ((kt & 3) << 29);
-          // Columns past K are zero in shared memory (TMA fills them), so a
-          // ragged last k-tile may run whole MMAs.
+          // Columns past K are zero in shared memory (TMA fills them), so a ragged
+          // last k-tile may run whole MMAs.
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const uint64_t a = sm100::desc_add(da, 32 * j), b = sm100::desc_add(db, 32 * j);
-            if constexpr (PAIR) sm100::mma_mxf8_ss_pair(d, a, b, idesc, sfa, sfb, (kt | j) != 0);
-            else sm100::mma_mxf8_ss(d, a, b, idesc, sfa, sfb, (kt | j) != 0);
+            if constexpr (PAIR) sm100::mma_mxf8_ss_pair(d, a, b, idesc, sfa, sfb + shift, (kt | j) != 0);
+            else sm100::mma_mxf8_ss(d, a, b, idesc, sfa, sfb + shift, (kt | j) != 0);
           }
           commit(&empty[stage]);
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
@@ -388,9 +403,9 @@ tile_kernel(const __grid_constant__ Maps maps, const Params p) {
     const uint32_t bias_addr = sm100::smem_u32(s_bias);
     int local = 0;
     uint32_t res_phase = 0;
-    // The bias of the warp's 64 columns passes through shared memory (each lane
-    // loads two and reads all); a tile's is loaded while the tile before it is
-    // waited for, its latency out of the way. So are the tile's coordinates.
+    // The bias of the warp's columns passes through shared memory (each lane
+    // loads two of 64 and reads all); a tile's is loaded while the tile before
+    // it is waited for, its latency out of the way. So are the coordinates.
     float bias0 = 0.0f, bias1 = 0.0f;
     Walk walk(p, tile0);
     int next_mb = 0, next_nb = 0;
@@ -1002,18 +1017,22 @@ struct Plan {
   int bt;        // rows kernel with BT rows of A per tile; 0: tile kernel
   int split;     // rows kernel: CTAs per tile along K
   int bn;        // tile kernel: columns per tile
-  bool pair;     // tile kernel: CTA pairs (256 x 256 tiles)
+  bool pair;     // tile kernel: CTA pairs (256-row tiles)
 };
 
 // Up to 32 rows run on the rows kernel, K split until two CTAs per SM have
 // work (measured, B200, us, split 1 / 2 / 4 / 8: 1 x 512 x 512 3.3 / 3.0 / 2.8
 // / -, 1 x 3072 x 3072 - / 4.9 / 4.1 / 4.2, 24 x 3072 x 14336 - / - / 14.0 /
 // 11.1; the tile kernel 4.1, 7.1 and 33). More rows take the tile kernel whose
-// waves cost less. Cycles of a k-tile and of a tile's hand-off, measured with
-// every SM busy: 400 and 300 on 128 x 128 tiles, 520 and 1300 on pairs, 620
-// and 1300 on 128 x 256, and 1500, 3000, 3000 for the last tile's epilogue
-// (3520 x 768 x 512: 5.0 us on 128 x 128 against 6.3 on pairs; 7040 x 3072 x
-// 3072 59 against 69 the other way).
+// waves cost least: cycles of a k-tile and of a tile's hand-over with every SM
+// busy, and of what comes before the first and after the last tile, fitted to
+// measurements. What they decide (us on 128 x 128 / pairs' 256 x 192 / 256 x
+// 256): 3520 x 768 x 512 6.1 / 6.5 / 7.3, 880 x 3072 x 3072 14.6 / 11.7 /
+// 13.9, 1759 x 3072 x 3072 22.1 / 18.3 / 22.0, 2500 x 4096 x 2048 27.0 / 21.6 /
+// 25.4, 300 x 9216 x 3072 17.1 / 18.3 / 15.5, 7040 x 3072 x 14336 318 / 250 /
+// 238. 128 x 128 tiles are bound by the operands' way into the SM (32 KB per
+// 256 cycles of MMA); 256 columns leave tensor memory for one accumulator
+// only, so their hand-over is not hidden.
 Plan plan_for(int M, int N, int K, bool swiglu) {
   const int sms = rc::sm_count(), k_tiles = fp8b::blocks_of(K);
   auto up = [](long long a, long long b) { return (a + b - 1) / b; };
@@ -1025,11 +1044,18 @@ Plan plan_for(int M, int N, int K, bool swiglu) {
     if (q.split > k_tiles) q.split = k_tiles;
     return q;
   }
-  const long long pair = up(up(M, 256) * up(N, 256), sms / 2) * (520LL * k_tiles + 1300) + 3000;
-  const long long one = swiglu ? up(up(M, 128) * up(N, 256), sms) * (620LL * k_tiles + 1300) + 3000
-                               : up(up(M, 128) * up(N, 128), sms) * (400LL * k_tiles + 300) + 1500;
-  q.pair = pair < one;
-  if (!q.pair && !swiglu) q.bn = 128;
+  struct Tile { int m, n, k_tile, tile, ends; };
+  auto cost = [&](const Tile& t) {
+    return up(up(M, t.m) * up(N, t.n), t.m == 256 ? sms / 2 : sms) * ((long long)t.k_tile * k_tiles + t.tile) + t.ends;
+  };
+  const long long pair = cost({256, 256, 520, 1300, 3000});
+  if (swiglu) {
+    q.pair = pair < cost({128, 256, 620, 1300, 3000});
+    return q;
+  }
+  const long long narrow = cost({256, 192, 420, 200, 4100}), one = cost({128, 128, 400, 300, 1500});
+  q.pair = pair < one || narrow < one;
+  q.bn = !q.pair ? 128 : narrow < pair ? 192 : 256;
   return q;
 }
 
@@ -1090,6 +1116,8 @@ template <int EPI, typename Out>
 int run(const Maps& maps, const Params& p, const Plan& q, cudaStream_t stream, const char* what) {
   if (q.bt == 16) return launch_rows<16, EPI, Out>(maps, p, q.split, stream, what);
   if (q.bt == 32) return launch_rows<32, EPI, Out>(maps, p, q.split, stream, what);
+  if constexpr (EPI == EPI_OUT)
+    if (q.bn == 192) return launch<192, 6, EPI, true, Out>(maps, p, stream, what);
   if (q.pair) return launch<256, EPI == EPI_OUT ? 5 : 6, EPI, true, Out>(maps, p, stream, what);
   if constexpr (EPI == EPI_OUT) return launch<128, 5, EPI, false, Out>(maps, p, stream, what);
   else return launch<256, 4, EPI, false, Out>(maps, p, stream, what);
@@ -1127,7 +1155,7 @@ int rc_fp8_block_gemm(const uint8_t* a, long long lda, const uint8_t* a_scales, 
   if (p.staged && !q.bt) {
     const auto type = out_dtype == fp8b::kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     const uint64_t dims[2] = {(uint64_t)N, (uint64_t)M};
-    const bool wide = q.bn == 256;                       // the warp's staging box (Smem::kBoxCols)
+    const bool wide = q.bn != 128;                       // the warp's staging box (Smem::kBoxCols)
     const uint32_t box[2] = {wide ? 32u : 64u, 32};
     const auto swizzle = wide ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
     const uint64_t so[1] = {(uint64_t)ldo * 2}, sr[1] = {(uint64_t)ldr * 2};
