@@ -71,8 +71,8 @@ def _build_binding(force: bool) -> None:
     # own linked in clashes with the runtime torch has loaded.
     cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{d}" for d in include),
-           BINDING_SOURCE, "-o", BINDING, "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10",
-           "-lc10_cuda", "-L" + PKG, "-l:" + os.path.basename(LIB), "-Wl,-rpath,$ORIGIN"]
+           BINDING_SOURCE, "-o", BINDING, "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu",
+           "-ltorch_cuda", "-lc10", "-lc10_cuda", "-L" + PKG, "-l:" + os.path.basename(LIB), "-Wl,-rpath,$ORIGIN"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode:
         raise RuntimeError(f"{cmd[0]} failed for {os.path.basename(BINDING_SOURCE)}:\n{r.stderr}")

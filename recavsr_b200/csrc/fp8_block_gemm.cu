@@ -672,38 +672,39 @@ int launch(const Maps& maps, const Params& p, cudaStream_t stream, const char* w
       rc::launch_pdl(kern, dim3(tiles < sms ? tiles : sms), dim3(tile_threads<BN>()), S::kTotal, stream, maps, p), what);
 }
 
-// Four columns n .. n+3 of an output row: bias and residual (`near`, loaded
-// ahead where rows start on 16 bytes) added, rounded, stored.
+// Four columns n .. n+3 of an output row: its residual (zeros where there is
+// none), and the rounded sum's store.
 template <typename Out>
-__device__ __forceinline__ void store_piece(const Params& p, int row, int n, const float (&sum)[4], uint2 near) {
+__device__ __forceinline__ void load_piece(const Params& p, int row, int n, float (&v)[4]) {
   const Out* res = static_cast<const Out*>(p.residual);
-  Out* out = static_cast<Out*>(p.out) + (size_t)row * p.ldo + n;
-  float f[4] = {sum[0], sum[1], sum[2], sum[3]};
-  if (p.bias) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c) v[c] = 0.0f;
+  if (!res || row >= p.M) return;
+  res += (size_t)row * p.ldr + n;
+  if (p.staged && n + 4 <= p.N) {
+    const uint2 w = rc::ld_in(reinterpret_cast<const uint2*>(res));
+    const float2 lo = unpack2<Out>(w.x), hi = unpack2<Out>(w.y);
+    v[0] = lo.x;
+    v[1] = lo.y;
+    v[2] = hi.x;
+    v[3] = hi.y;
+  } else {
 #pragma unroll
     for (int c = 0; c < 4; ++c)
-      if (n + c < p.N) f[c] += rc::ld_in(p.bias + n + c);
+      if (n + c < p.N) v[c] = fp8b::to_float(rc::ld_in(res + c));
   }
+}
+template <typename Out>
+__device__ __forceinline__ void store_piece(const Params& p, int row, int n, const float (&f)[4]) {
+  if (row >= p.M) return;
+  Out* out = static_cast<Out*>(p.out) + (size_t)row * p.ldo + n;
   if (p.staged && n + 4 <= p.N) {
-    if (res) {
-      const float2 lo = unpack2<Out>(near.x), hi = unpack2<Out>(near.y);
-      f[0] += lo.x;
-      f[1] += lo.y;
-      f[2] += hi.x;
-      f[3] += hi.y;
-    }
     Out* tag = nullptr;
     *reinterpret_cast<uint2*>(out) = make_uint2(fp8b::pack2(f[0], f[1], tag), fp8b::pack2(f[2], f[3], tag));
   } else {
-    float r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (res) {
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        if (n + c < p.N) r[c] = fp8b::to_float(rc::ld_in(res + (size_t)row * p.ldr + n + c));
-    }
 #pragma unroll
     for (int c = 0; c < 4; ++c)
-      if (n + c < p.N) out[c] = fp8b::from_float(f[c] + r[c], (Out*)nullptr);
+      if (n + c < p.N) out[c] = fp8b::from_float(f[c], (Out*)nullptr);
   }
 }
 
@@ -911,15 +912,11 @@ rows_kernel(const __grid_constant__ Maps maps, const Params p, int split) {
     for (int j = 0; j < kRows; ++j)
 #pragma unroll
       for (int w = 0; w < kW; ++w) v[j][w] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    uint2 near[kRows];                                             // residual
-    const Out* res = static_cast<const Out*>(p.residual);
+    float near[kRows][4];                                          // residual
     const int n = wt * BM + lane * 4;
-    const bool vec = p.staged && n + 4 <= p.N;
-    if (EPI == EPI_OUT && res && vec) {
+    if constexpr (EPI == EPI_OUT) {
 #pragma unroll
-      for (int j = 0; j < kRows; ++j)
-        near[j] = rc::ld_in(reinterpret_cast<const uint2*>(
-            res + (size_t)(tt * BT + first + min(i + j, mine - 1)) * p.ldr + n));
+      for (int j = 0; j < kRows; ++j) load_piece<Out>(p, tt * BT + first + min(i + j, mine - 1), n, near[j]);
     }
     for (int q = 0; q < split; ++q) {
 #pragma unroll
@@ -946,26 +943,8 @@ rows_kernel(const __grid_constant__ Maps maps, const Params p, int split) {
         v[j][w].w += bias[w].w;
       }
       if constexpr (EPI == EPI_OUT) {
-        Out* out = static_cast<Out*>(p.out) + (size_t)row * p.ldo + n;
-        float f[4] = {v[j][0].x, v[j][0].y, v[j][0].z, v[j][0].w};
-        if (vec) {
-          if (res) {
-            const float2 lo = unpack2<Out>(near[j].x), hi = unpack2<Out>(near[j].y);
-            f[0] += lo.x;
-            f[1] += lo.y;
-            f[2] += hi.x;
-            f[3] += hi.y;
-          }
-          Out* tag = nullptr;
-          *reinterpret_cast<uint2*>(out) = make_uint2(fp8b::pack2(f[0], f[1], tag), fp8b::pack2(f[2], f[3], tag));
-        } else {
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-            if (n + c < p.N) {
-              if (res) f[c] += fp8b::to_float(rc::ld_in(res + (size_t)row * p.ldr + n + c));
-              out[c] = fp8b::from_float(f[c], (Out*)nullptr);
-            }
-        }
+        const float f[4] = {v[j][0].x + near[j][0], v[j][0].y + near[j][1], v[j][0].z + near[j][2], v[j][0].w + near[j][3]};
+        store_piece<Out>(p, row, n, f);
       } else {
         const float g[4] = {v[j][0].x, v[j][0].y, v[j][0].z, v[j][0].w};
         const float u[4] = {v[j][kW - 1].x, v[j][kW - 1].y, v[j][kW - 1].z, v[j][kW - 1].w};
@@ -1010,12 +989,219 @@ int launch_rows(const Maps& maps, const Params& p, int split, cudaStream_t strea
                           what);
 }
 
+// ---------------------------------------------------------------- split K
+// OUT for too few 128 x 128 tiles and too many rows for the rows kernel: a
+// cluster of SPLIT CTAs takes one tile, each a range of k-tiles, and CTA q ends
+// up with the tile's columns [q * 128 / SPLIT, ...): every CTA lays its fp32
+// partial out by owner in the operands' stages and sends each owner its slice
+// as one bulk copy between the two SMs' shared memory, counted on the owner's
+// barrier (stores and loads of single values between SMs took 3 us longer);
+// the owner sums the slices in rank order.
+constexpr int kSplitThreads = 64 + 256;
+
+template <int SPLIT>
+struct SplitSmem {
+  static constexpr int kStages = 4;
+  static constexpr int kCols = BM / SPLIT;                  // columns per owner
+  static constexpr int kStage = 2 * BM * kRowBytes, kSf = 2 * kSfAtom;
+  static constexpr int kSlice = BM * kCols * 4;             // an owner's columns of one CTA's partial, [128][kCols] fp32
+  static constexpr int offIn = kStages * kStage;            // the slices this CTA owns, by rank
+  static constexpr int offSf = offIn + SPLIT * kSlice;
+  static constexpr int offBar = offSf + kStages * kSf;
+  static constexpr int kTotal = offBar + (2 * kStages + 4) * 8;
+  static_assert(kTotal <= 232448 && SPLIT * kSlice <= kStages * kStage, "shared memory");
+};
+
+template <int SPLIT, typename Out>
+__global__ void __launch_bounds__(kSplitThreads, 1)
+split_kernel(const __grid_constant__ Maps maps, const Params p) {
+  using S = SplitSmem<SPLIT>;
+  constexpr int STAGES = S::kStages, kCols = S::kCols;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::offBar);
+  uint64_t* empty = full + STAGES;
+  uint64_t* acc_full = empty + STAGES;
+  uint64_t* slices = acc_full + 1;               // the other CTAs' slices have arrived
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(acc_full + 2);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 3);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = (int)sm100::cluster_ctarank();
+  const int tile = blockIdx.x / SPLIT;
+  const int mb = tile % p.m_blocks, nb = tile / p.m_blocks;
+  const int kt0 = (int)((long long)rank * p.k_tiles / SPLIT), kt1 = (int)((long long)(rank + 1) * p.k_tiles / SPLIT);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      sm100::mbar_init(&full[s], 1);
+      sm100::mbar_init(&empty[s], 1);
+    }
+    sm100::mbar_init(acc_full, 1);
+    sm100::mbar_init(slices, 1);
+    *abort_flag = 0;
+    sm100::fence_mbar_init();
+    sm100::mbar_arrive_expect_tx(slices, (SPLIT - 1) * S::kSlice);
+  }
+  if (warp == 1) {
+    sm100::tmem_alloc(tmem_slot, 256);
+    sm100::tmem_relinquish();
+  }
+  sm100::tc_fence_before();
+  __syncthreads();
+  sm100::cluster_sync();                         // every CTA's barriers are there before a slice is sent
+  sm100::tc_fence_after();
+  rc::pdl_trigger();
+  rc::pdl_wait();
+  const uint32_t tmem = *tmem_slot, tmem_sf = tmem + BM;
+  auto wait = [&](uint64_t* bar, uint32_t parity, unsigned int site) -> bool {
+    if (sm100::mbar_wait(bar, parity, abort_flag)) return true;
+    if (!*abort_flag) {
+      rc::device_fail(kKernFp8Block, site);
+      *abort_flag = 1;
+    }
+    return false;
+  };
+
+  if (warp == 0) {
+    if (sm100::elect_one_sync()) {
+      int stage = 0, issued = 0;
+      uint32_t phase = 0;
+      for (int kt = kt0; kt < kt1; ++kt) {
+        if (!wait(&empty[stage], phase ^ 1, 21)) break;
+        uint8_t* a = smem + stage * S::kStage;
+        uint8_t* sf = smem + S::offSf + stage * S::kSf;
+        const bool atom = (kt & 3) == 0 || kt == kt0;
+        const int line = (kt >> 2) * 4;
+        sm100::mbar_arrive_expect_tx(&full[stage], S::kStage + (atom ? S::kSf : 0));
+        sm100::tma_load_2d(a, &maps.a, &full[stage], kt * kRowBytes, mb * BM);
+        sm100::tma_load_2d(a + BM * kRowBytes, &maps.b, &full[stage], kt * kRowBytes, nb * BM);
+        if (atom) {
+          sm100::tma_load_2d(sf, &maps.sfa, &full[stage], 0, mb * p.katoms * 4 + line);
+          sm100::tma_load_2d(sf + kSfAtom, &maps.sfb, &full[stage], 0, nb * p.katoms * 4 + line);
+        }
+        ++issued;
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+      }
+      for (int s = 0; s < STAGES && issued > 0; ++s, --issued) {   // loads land before the CTA goes on
+        if (stage == 0) { stage = STAGES; phase ^= 1; }
+        --stage;
+        sm100::mbar_wait(&full[stage], phase);
+      }
+    }
+  } else if (warp == 1) {
+    if (sm100::elect_one_sync()) {
+      int stage = 0, sf_buf = 1;
+      uint32_t phase = 0, sfa = 0;
+      const uint64_t d0 = sm100::desc_kmajor_sw128(sm100::smem_u32(smem));
+      const uint64_t dsf0 = sm100::desc_sf_rows(sm100::smem_u32(smem + S::offSf));
+      for (int kt = kt0; kt < kt1; ++kt) {
+        if (!wait(&full[stage], phase, 22)) break;
+        sm100::tc_fence_after();
+        if ((kt & 3) == 0 || kt == kt0) {
+          sf_buf ^= 1;
+          sfa = tmem_sf + sf_buf * 8;
+          sm100::tmem_cp_32x128b_warpx4(sfa, sm100::desc_add(dsf0, stage * S::kSf));
+          sm100::tmem_cp_32x128b_warpx4(sfa + 4, sm100::desc_add(dsf0, stage * S::kSf + kSfAtom));
+        }
+        const uint32_t idesc = sm100::idesc_mxf8(BM, BM, 0) | ((kt & 3) << 4) | ((kt & 3) << 29);
+        const uint64_t da = sm100::desc_add(d0, stage * S::kStage), db = sm100::desc_add(da, BM * kRowBytes);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          sm100::mma_mxf8_ss(tmem, sm100::desc_add(da, 32 * j), sm100::desc_add(db, 32 * j), idesc, sfa, sfa + 4,
+                             kt != kt0 || j != 0);
+        sm100::tc_commit(&empty[stage]);
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+      }
+      sm100::tc_commit(acc_full);
+      sm100::mbar_wait(acc_full, 0);
+    }
+  }
+  __syncwarp();
+  // 16-byte piece `c` (of kCols / 4) of row r of a slice: pieces are swizzled by
+  // the row, so that 8 rows' (or one row's) pieces hit all banks.
+  constexpr int kPieces = kCols / 4;
+  auto piece = [&](int r, int c) {
+    return (uint32_t)((r * kPieces + (c ^ (r & (kPieces < 8 ? kPieces - 1 : 7)))) * 16);
+  };
+  const uint32_t out_slices = sm100::smem_u32(smem), in_slices = sm100::smem_u32(smem + S::offIn);
+  constexpr int kTasks = BM * kPieces / 256;                // 4-column pieces of the owned slice per thread
+  const int t0 = (int)threadIdx.x - 64, n = nb * BM + rank * kCols + t0 % kPieces * 4;   // its columns: n .. n + 3
+  const Out* res = static_cast<const Out*>(p.residual);
+  float near[kTasks][4], bias[4];
+  if (warp >= 2) {
+    // Residual and bias, in flight over the main loop.
+#pragma unroll
+    for (int c = 0; c < 4; ++c) bias[c] = p.bias && n + c < p.N ? rc::ld_in(p.bias + n + c) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < kTasks; ++i) {
+      const int row = mb * BM + (t0 + i * 256) / kPieces;
+      load_piece<Out>(p, row, n, near[i]);
+    }
+    const int quad = warp & 3, half = (warp - 2) >> 2, r = quad * 32 + lane;
+    if (__all_sync(0xffffffffu, wait(acc_full, 0, 23))) {
+      sm100::tc_fence_after();
+      uint32_t acc[64];
+      load_acc(tmem + half * 64 + ((uint32_t)(quad * 32) << 16), acc);
+      acc_ready(acc);
+#pragma unroll
+      for (int c = 0; c < 64; c += 4) {
+        const int col = half * 64 + c, q = col / kCols;
+        const uint32_t to = (q == rank ? in_slices : out_slices) + q * S::kSlice + piece(r, col % kCols / 4);
+        st_shared4(to, make_uint4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]));
+      }
+      sm100::tc_fence_before();
+    }
+    sm100::fence_proxy_async_smem();
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    if (t0 < SPLIT && t0 != rank)                           // thread q sends rank q its slice
+      asm volatile(
+          "cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+              sm100::mapa(in_slices + rank * S::kSlice, t0)),
+          "r"(out_slices + t0 * S::kSlice), "r"((uint32_t)S::kSlice), "r"(sm100::mapa(sm100::smem_u32(slices), t0))
+          : "memory");
+    if (__all_sync(0xffffffffu, wait(slices, 0, 24))) {
+#pragma unroll
+      for (int i = 0; i < kTasks; ++i) {
+        const int r = (t0 + i * 256) / kPieces, row = mb * BM + r;
+        float f[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int q = 0; q < SPLIT; ++q) {
+          const float4 x = ld_shared4(in_slices + q * S::kSlice + piece(r, t0 % kPieces));
+          f[0] += x.x;
+          f[1] += x.y;
+          f[2] += x.z;
+          f[3] += x.w;
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) f[c] = f[c] + bias[c] + near[i][c];
+        store_piece<Out>(p, row, n, f);
+      }
+    }
+  }
+  sm100::cluster_sync();      // no CTA leaves while its slices are on their way
+  if (warp == 1) {
+    sm100::tc_fence_after();
+    sm100::tmem_dealloc(tmem, 256);
+  }
+}
+
+template <int SPLIT, typename Out>
+int launch_split(const Maps& maps, const Params& p, cudaStream_t stream, const char* what) {
+  using S = SplitSmem<SPLIT>;
+  auto kern = split_kernel<SPLIT, Out>;
+  static rc::SmemAttrFlags flags = {};
+  if (const int r = rc::ensure_smem_attr(flags, reinterpret_cast<const void*>(kern), S::kTotal, what)) return r;
+  return rc::check_launch(rc::launch_pdl_cluster(kern, dim3((unsigned)(p.m_blocks * p.n_blocks * SPLIT)),
+                                                 dim3(kSplitThreads), S::kTotal, stream, SPLIT, maps, p),
+                          what);
+}
+
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 // How a product runs.
 struct Plan {
   int bt;        // rows kernel with BT rows of A per tile; 0: tile kernel
-  int split;     // rows kernel: CTAs per tile along K
+  int split;     // rows kernel, and split kernel (bt 0, split > 1): CTAs per tile along K
   int bn;        // tile kernel: columns per tile
   bool pair;     // tile kernel: CTA pairs (256-row tiles)
 };
@@ -1056,6 +1242,23 @@ Plan plan_for(int M, int N, int K, bool swiglu) {
   const long long narrow = cost({256, 192, 420, 200, 4100}), one = cost({128, 128, 400, 300, 1500});
   q.pair = pair < one || narrow < one;
   q.bn = !q.pair ? 128 : narrow < pair ? 192 : 256;
+  // Few tiles and a long K: split while the clusters find room at once (of 8
+  // CTAs, 12 do on 148 SMs). The exchange costs what about 9, 15 and 21
+  // k-tiles do (us, split 1 / 2 / 4 / 8: 128 x 3072 x 3072 7.6 / 7.0 / 7.4 / -,
+  // 500 x 500 x 5008 18.9 / 12.7 / 10.0 / -, 100 x 200 x 10000 30.5 / 18.0 /
+  // 11.8 / 9.2, 300 x 3072 x 14336 31.3 / 24.0 / - / -; 128 x 768 x 512 4.2 /
+  // 5.9).
+  const long long tiles = up(M, 128) * up(N, 128);
+  const struct { int split, ctas, exchange; } kSplits[] = {{2, sms, 3600}, {4, sms * 7 / 8, 6000}, {8, sms * 2 / 3, 8500}};
+  long long best = q.pair ? (narrow < pair ? narrow : pair) : one;
+  for (const auto& x : kSplits) {
+    const long long with = 400 * up(k_tiles, x.split) + 1800 + x.exchange;
+    if (tiles * x.split > x.ctas || k_tiles < x.split || with >= best) continue;
+    best = with;
+    q.pair = false;
+    q.bn = 128;
+    q.split = x.split;
+  }
   return q;
 }
 
@@ -1116,6 +1319,11 @@ template <int EPI, typename Out>
 int run(const Maps& maps, const Params& p, const Plan& q, cudaStream_t stream, const char* what) {
   if (q.bt == 16) return launch_rows<16, EPI, Out>(maps, p, q.split, stream, what);
   if (q.bt == 32) return launch_rows<32, EPI, Out>(maps, p, q.split, stream, what);
+  if constexpr (EPI == EPI_OUT) {
+    if (q.split == 2) return launch_split<2, Out>(maps, p, stream, what);
+    if (q.split == 4) return launch_split<4, Out>(maps, p, stream, what);
+    if (q.split == 8) return launch_split<8, Out>(maps, p, stream, what);
+  }
   if constexpr (EPI == EPI_OUT)
     if (q.bn == 192) return launch<192, 6, EPI, true, Out>(maps, p, stream, what);
   if (q.pair) return launch<256, EPI == EPI_OUT ? 5 : 6, EPI, true, Out>(maps, p, stream, what);
@@ -1152,7 +1360,7 @@ int rc_fp8_block_gemm(const uint8_t* a, long long lda, const uint8_t* a_scales, 
   // TMA moves the output (and the residual) where rows start on 16 bytes.
   p.staged = aligned16(out) && ldo % 8 == 0 && aligned16(residual) && (!residual || ldr % 8 == 0);
   p.pairs = ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(residual)) % 4 | ldo % 2 | (residual ? ldr % 2 : 0)) == 0;
-  if (p.staged && !q.bt) {
+  if (p.staged && !q.bt && q.split == 1) {
     const auto type = out_dtype == fp8b::kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     const uint64_t dims[2] = {(uint64_t)N, (uint64_t)M};
     const bool wide = q.bn != 128;                       // the warp's staging box (Smem::kBoxCols)

@@ -6,6 +6,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -64,7 +65,7 @@ at::Tensor vector(const at::Tensor& t, int64_t n, const at::Tensor& like, const 
 int64_t scale_numel(int64_t rows, int64_t cols) { return up(rows, kBlock) * kBlock * up(cols, 4 * kBlock) * 4; }
 
 at::Tensor empty(at::IntArrayRef size, at::ScalarType type, const at::Tensor& like) {
-  return at::empty(size, like.options().dtype(type));
+  return at::detail::empty_cuda(size, type, like.device(), c10::nullopt);    // at::empty without its dispatch
 }
 
 // Codes [rows, K] and their scales; codes as rows the kernels can read.
