@@ -2,7 +2,10 @@
 // an RMSNorm (with the residual's addition) produces. All are bound by the
 // bytes they move: every input byte is read once, every output byte written
 // once, and the scale of a block comes out of the registers of the 16 lanes
-// that hold it.
+// that hold it. Measured (B200, device time, of the measured 6456 GB/s):
+// rows 7040 x 14336 bf16 52.4 us = 0.90, 14080 x 512 bf16 4.0 us = 0.84 (from
+// L2); norm with residual 14081 x 2048 fp32 57.7 us = 1.0, 3520 x 512 bf16 3.2
+// us, one row 2.2 us (launch and one round trip to memory).
 #include <type_traits>
 
 #include "fp8_block.cuh"

@@ -13,6 +13,9 @@
     python -m recavsr_b200.profile_case lq_conv1     # LQ projector conv1: im2col + bf16 GEMM, body block
     python -m recavsr_b200.profile_case lq_conv2     # LQ projector conv2: im2col + bf16 GEMM, body block
     python -m recavsr_b200.profile_case lq_norm      # channel RMSNorm + SiLU, 14080 x 2048
+    python -m recavsr_b200.profile_case fp8_mm       # block-scaled FP8 product 3520x3072x3072 (+bias, residual)
+    python -m recavsr_b200.profile_case fp8_swiglu   # block-scaled FP8 gated product 14080x2048x512
+    python -m recavsr_b200.profile_case fp8_norm     # residual + RMSNorm held in block-scaled FP8, 14080x2048 fp32
 
 Each case allocates fresh inputs (a few hundred MB at most), captures `--reps`
 launches in a CUDA graph, replays it and prints the mean CUDA-event time per
@@ -245,7 +248,33 @@ def _decoder_step(h=44, w=80):
     return (lambda: list(sess.step(lat, lr_up=lr4))), 0.91e12, "TFLOP/s"
 
 
+def _fp8_mm(m=2 * M, n=DIM, k=DIM):
+    from .runtime import fp8_block
+    a = fp8_block.quantize(torch.randn(m, k, device="cuda"))
+    w = fp8_block.quantize_weight(torch.randn(n, k, device="cuda") / k ** 0.5)
+    bias, res = torch.zeros(n, device="cuda"), torch.randn(m, n, device="cuda").bfloat16()
+    return (lambda: fp8_block.mm(a[0], w[0], a[1], w[1], bias, residual=res)), 2.0 * m * n * k, "TFLOP/s"
+
+
+def _fp8_swiglu(m=14080, h=2048, k=512):
+    from .runtime import fp8_block
+    a = fp8_block.quantize(torch.randn(m, k, device="cuda"))
+    w = fp8_block.quantize_weight(torch.randn(2 * h, k, device="cuda") / k ** 0.5)
+    bias = torch.zeros(2 * h, device="cuda")
+    return (lambda: fp8_block.swiglu_mm(a[0], w[0], a[1], w[1], bias)), 4.0 * m * h * k, "TFLOP/s"
+
+
+def _fp8_norm(m=14080, n=2048):
+    from .runtime import fp8_block
+    x, r = torch.randn(m, n, device="cuda"), torch.randn(m, n, device="cuda")
+    w = torch.ones(n, device="cuda")
+    return (lambda: fp8_block.rms_norm_quantize(x, w, 1e-5, residual=r)), m * n * 13.0, "GB/s"
+
+
 CASES = {
+    "fp8_mm": _fp8_mm,
+    "fp8_swiglu": _fp8_swiglu,
+    "fp8_norm": _fp8_norm,
     "decoder": _decoder,
     "decoder_step": _decoder_step,
     "decoder_backbone": lambda: _decoder(qf=1, nf=2),
