@@ -782,6 +782,7 @@ rows_kernel(const __grid_constant__ Maps maps, const Params p, int split) {
   }
   sm100::tc_fence_before();
   __syncthreads();
+  sm100::cluster_arrive();      // this CTA runs; waited for before the first store into a peer
   sm100::tc_fence_after();
   rc::pdl_trigger();
   rc::pdl_wait();
@@ -865,6 +866,7 @@ rows_kernel(const __grid_constant__ Maps maps, const Params p, int split) {
     ok = __all_sync(0xffffffffu, wait(acc_full, 0, 13));
     sm100::tc_fence_after();
   }
+  sm100::cluster_wait();        // every CTA of the cluster runs: their shared memory may be written
   if (warp >= 2 && ok) {
     const int quad = warp & 3;
     constexpr int kChunk = BT < 32 ? BT : 32;
