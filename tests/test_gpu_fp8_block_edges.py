@@ -1,11 +1,12 @@
 """Block-scaled FP8 operators at their edges: few rows with K over a cluster,
-gates far below zero, operands and outputs that are refused.
+special values, strides and middle row counts of the gated product.
 
 Tolerances of the products: tests/test_gpu_fp8_block.py."""
 import pytest
 import torch
 
-from tests.test_gpu_fp8_block import assert_rounded_from, check_mm, check_swiglu, operands, sum_slack
+from tests.test_gpu_fp8_block import (activations, assert_rounded_from, check_mm, check_swiglu, held, operands,
+                                      sum_slack)
 from tests.util import assert_no_device_error
 
 pytestmark = pytest.mark.gpu
@@ -38,3 +39,47 @@ def test_few_rows_back_to_back(n, k):
     for out in outs[1:]:
         assert torch.equal(out, outs[0])
     assert_no_device_error()
+
+
+# ---------------------------------------------------------------- gated product
+@pytest.mark.parametrize("m", [3, 30, 200])
+def test_swiglu_special_values(m):
+    """A NaN or an infinity of the operands marks the row's blocks that it reaches; zero rows stay zero."""
+    from recavsr_b200.runtime import fp8_block
+    k, h = 256, 256
+    x = activations(m, k, torch.float32, 42)
+    clean = x.clone()
+    clean[0] = 0
+    x[0], x[1, 3], x[2, 200] = 0, float("nan"), float("inf")
+    w = fp8_block.quantize_weight(fp8_block.interleave_gate_up(*activations(2 * h, k, torch.float32, 43).chunk(2)))
+    (ac, asc), (bc, bsc) = fp8_block.quantize(x), fp8_block.quantize(clean)
+    codes, scales = fp8_block.swiglu_mm(ac, w[0], asc, w[1])
+    want, want_scales = fp8_block.swiglu_mm(bc, w[0], bsc, w[1])
+    c, e = held(codes, scales)
+    wc, we = held(want, want_scales)
+    assert not (c[0] & 0x7f).any() and (e[0] == 1).all()
+    for row in (1, 2):
+        assert (c[row] == 0x7f).all() and (e[row] == 255).all()
+    rest = [i for i in range(m) if i not in (1, 2)]
+    assert (c[rest] == wc[rest]).all() and (e[rest] == we[rest]).all()
+
+
+@pytest.mark.parametrize("m,h,k", [(33, 1024, 4096), (100, 1040, 2064), (256, 2048, 4096), (520, 528, 1536),
+                                   (900, 1024, 2048)])
+def test_swiglu_middle_rows(m, h, k):
+    check_swiglu(m, h, k)
+    assert_no_device_error()
+
+
+@pytest.mark.parametrize("m", [5, 200])
+def test_swiglu_strided_codes(m):
+    """Codes as columns of wider buffers, on and off 16 bytes."""
+    from recavsr_b200.runtime import fp8_block
+    ac, asc = fp8_block.quantize(activations(m, 256, torch.float32, 44))
+    wc, wsc = fp8_block.quantize_weight(activations(256, 256, torch.float32, 45))
+    want = fp8_block.swiglu_mm(ac, wc, asc, wsc)
+    for cols, at in ((512, 64), (300, 3)):
+        wide, weight = (torch.zeros(t.shape[0], cols, dtype=torch.uint8, device="cuda") for t in (ac, wc))
+        wide[:, at:at + 256], weight[:, at:at + 256] = ac, wc
+        got = fp8_block.swiglu_mm(wide[:, at:at + 256], weight[:, at:at + 256], asc, wsc)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
