@@ -112,51 +112,23 @@ __device__ __forceinline__ float2 unpack2(uint32_t w) {
   else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 
-// silu(g) * u with the MUFU exp2 and reciprocal (relative error under 2^-20,
-// far below the E4M3 rounding that follows).
-__device__ __forceinline__ float swiglu(float g, float u) {
-  float e, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-  return g * r * u;
-}
-// 2^z for a pair on the FMA pipe: z = j + f with j = rint(z) and |f| <= 1/2, a
-// degree-5 polynomial for 2^f (coefficients fitted here, relative error
-// 2.1e-7) and j added to the exponent field. z is clamped to [-126, 127]: past
-// either end 1 + 2^z has long become 1, or its reciprocal been flushed to 0.
-__device__ __forceinline__ float2 exp2_fma(float2 z) {
-  constexpr float kRound = 12582912.0f;            // 1.5 * 2^23
-  const float2 zc = make_float2(fminf(fmaxf(z.x, -126.0f), 127.0f), fminf(fmaxf(z.y, -126.0f), 127.0f));
-  const float2 t = __fadd2_rn(zc, make_float2(kRound, kRound));
-  const float2 j = __fadd2_rn(t, make_float2(-kRound, -kRound));
-  const float2 f = __ffma2_rn(j, make_float2(-1.0f, -1.0f), zc);
-  constexpr float c5 = 0.00132764701f, c4 = 0.00967554096f, c3 = 0.0555071346f, c2 = 0.240221202f,
-                  c1 = 0.693146944f, c0 = 1.00000012f;
-  float2 q = __ffma2_rn(make_float2(c5, c5), f, make_float2(c4, c4));
-  q = __ffma2_rn(q, f, make_float2(c3, c3));
-  q = __ffma2_rn(q, f, make_float2(c2, c2));
-  q = __ffma2_rn(q, f, make_float2(c1, c1));
-  q = __ffma2_rn(q, f, make_float2(c0, c0));
-  return make_float2(__uint_as_float(__float_as_uint(q.x) + (__float_as_uint(t.x) << 23)),
-                     __uint_as_float(__float_as_uint(q.y) + (__float_as_uint(t.y) << 23)));
-}
-// silu(g) * u of a pair; the MUFU evaluates the exp2, or (FMA) the polynomial.
-// At two MUFU results per output the MUFU would take as long as the MMAs of a
-// 512-long K, so part of the exp2s run on the FMA pipe.
-template <bool FMA>
+// silu(g) u of a pair as g / (1 + t) p u p with t = s^2 = exp(-|g|): p = 1 where
+// g >= 0, and s below, where silu(g) = g t / (1 + t). The exponential of the half
+// argument stays in range (s down to g = -174, silu under 2^-243) where exp(-g)
+// would overflow, or its reciprocal flush, from g = -87 on; multiplied in one at
+// a time, p keeps the product out of the subnormals until the last step. The MUFU
+// evaluates exp2 and the reciprocal: the relative error is under 2^-19 + |g|
+// 2^-23, the second part that of g rounded once more (the argument of exp2 is).
 __device__ __forceinline__ float2 swiglu2(float2 g, float2 u) {
-  const float2 z = __fmul2_rn(g, make_float2(-1.4426950408889634f, -1.4426950408889634f));
-  float2 e, r;
-  if constexpr (FMA) {
-    e = exp2_fma(z);
-  } else {
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(z.x));
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(z.y));
-  }
-  const float2 d = __fadd2_rn(e, make_float2(1.0f, 1.0f));
+  constexpr float kHalfLog2e = 0.72134752044448170f;
+  float2 s, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(s.x) : "f"(fabsf(g.x) * -kHalfLog2e));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(s.y) : "f"(fabsf(g.y) * -kHalfLog2e));
+  const float2 d = __ffma2_rn(s, s, make_float2(1.0f, 1.0f));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(d.x));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(d.y));
-  return __fmul2_rn(__fmul2_rn(g, r), u);
+  const float2 p = make_float2(g.x < 0.0f ? s.x : 1.0f, g.y < 0.0f ? s.y : 1.0f);
+  return __fmul2_rn(__fmul2_rn(__fmul2_rn(__fmul2_rn(g, r), p), u), p);
 }
 
 // Columns of this thread's accumulator row into registers, complete on return.
@@ -599,7 +571,7 @@ tile_kernel(const __grid_constant__ Maps maps, const Params p) {
                                           i ? make_float2(bg.z, bg.w) : make_float2(bg.x, bg.y));
               const float2 u = __fadd2_rn(make_float2(__uint_as_float(acc[32 + c + i]), __uint_as_float(acc[33 + c + i])),
                                           i ? make_float2(bu.z, bu.w) : make_float2(bu.x, bu.y));
-              const float2 v = i == 2 && c % 8 == 4 ? swiglu2<true>(g, u) : swiglu2<false>(g, u);
+              const float2 v = swiglu2(g, u);
               y[c + i] = v.x;
               y[c + i + 1] = v.y;
             }
@@ -959,14 +931,15 @@ rows_kernel(const __grid_constant__ Maps maps, const Params p, int split) {
         const float f[4] = {v[j][0].x + near[j][0], v[j][0].y + near[j][1], v[j][0].z + near[j][2], v[j][0].w + near[j][3]};
         store_piece<Out>(p, row, n, f);
       } else {
-        const float g[4] = {v[j][0].x, v[j][0].y, v[j][0].z, v[j][0].w};
-        const float u[4] = {v[j][kW - 1].x, v[j][kW - 1].y, v[j][kW - 1].z, v[j][kW - 1].w};
-        float y[4];
+        const float4 g = v[j][0], u = v[j][kW - 1];
+        const float2 lo = swiglu2(make_float2(g.x, g.y), make_float2(u.x, u.y));
+        const float2 hi = swiglu2(make_float2(g.z, g.w), make_float2(u.z, u.w));
+        float y[4] = {lo.x, lo.y, hi.x, hi.y};
         const int col = wt * 128 + lane * 4;
         uint32_t m = 0;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          y[c] = col < p.H ? swiglu(g[c], u[c]) : 0.0f;      // H is a multiple of 16
+          if (col >= p.H) y[c] = 0.0f;                       // H is a multiple of 16
           m = max(m, fp8b::magnitude(y[c]));
         }
         const uint32_t e = fp8b::scale_byte(__reduce_max_sync(0xffffffffu, m));

@@ -1,12 +1,13 @@
 """Block-scaled FP8 operators at their edges: few rows with K over a cluster,
-special values, strides and middle row counts of the gated product.
+gates far below zero, special values, strides and middle row counts of the gated
+product.
 
 Tolerances of the products: tests/test_gpu_fp8_block.py."""
 import pytest
 import torch
 
-from tests.test_gpu_fp8_block import (activations, assert_rounded_from, check_mm, check_swiglu, held, operands,
-                                      sum_slack)
+from tests.test_gpu_fp8_block import (activations, assert_held_near, assert_rounded_from, check_mm, check_swiglu, f64,
+                                      held, operands, sum_slack)
 from tests.util import assert_no_device_error
 
 pytestmark = pytest.mark.gpu
@@ -38,6 +39,43 @@ def test_few_rows_back_to_back(n, k):
     assert_rounded_from(outs[0], av @ bv.t(), sum_slack(av, bv, k))
     for out in outs[1:]:
         assert torch.equal(out, outs[0])
+    assert_no_device_error()
+
+
+# ---------------------------------------------------------------- gates far from zero
+# Instruction errors of silu(g) u = g / (1 + t) * p * u * p with t = s^2 = exp(-|g|) and p = s below zero, else 1:
+# s carries 2^-22 of the exponential and |g| / 2 (2^-24 + 2^-26) of its rounded argument, both twice in p p and once
+# more at most through 1 + t; the reciprocal and five roundings add 2^-23 + 5 2^-24: under 2^-19 + |g| 2^-23.
+def gated_reference(g, u, dg, du):
+    """silu(g) u in 64 bits, and how far off it may be when g and u are known to within dg and du."""
+    sigma = torch.sigmoid(g)
+    y = g * sigma * u
+    # |silu'| <= sigma (1 + |g|) and sigma grows by at most exp(dg) over dg
+    slack = 1.01 * sigma * (1 + g.abs()) * dg * u.abs() + (g * sigma).abs() * du
+    return y, slack + (2.0 ** -19 + g.abs() * 2.0 ** -23) * y.abs() + 2.0 ** -148
+
+
+@pytest.mark.parametrize("m", [2, 20, 40, 300])
+def test_swiglu_gates_far_below_zero(m):
+    """Whole blocks of 128 outputs with gates about -10 to -150 (and one of large
+    positive ones): fp32 holds exp(-|g|) of the first five, and the square root
+    of the others'; an 8-bit block holds values down to 2^-136."""
+    from recavsr_b200.runtime import fp8_block
+    k, gates = 256, [-10.0, -30.0, -60.0, -80.0, -86.0, -90.0, -93.0, -150.0, 40.0]
+    h = 128 * len(gates)
+    gen = torch.Generator("cuda").manual_seed(41)
+    rand = lambda *s: torch.randn(*s, device="cuda", generator=gen)
+    ac, asc = fp8_block.quantize(rand(m, k))
+    wc, wsc = fp8_block.quantize_weight(fp8_block.interleave_gate_up(rand(h, k) / k ** 0.5, rand(h, k) / k ** 0.5))
+    bg = torch.tensor(gates, device="cuda").repeat_interleave(128)
+    bu = rand(h)
+    got = fp8_block.swiglu_mm(ac, wc, asc, wsc, fp8_block.interleave_gate_up(bg, bu), features=h)
+    av = fp8_block.dequantize(ac, asc).double()
+    wv = fp8_block.dequantize(wc, wsc).double().view(-1, 2, 128, k)
+    gv, uv = wv[:, 0].reshape(-1, k), wv[:, 1].reshape(-1, k)
+    g, u = av @ gv.t() + bg.double(), av @ uv.t() + bu.double()
+    y, slack = gated_reference(g, u, *(sum_slack(av, v, k) + 2.0 ** -22 * t.abs() for v, t in ((gv, g), (uv, u))))
+    assert_held_near(*got, f64(y), f64(slack))
     assert_no_device_error()
 
 
