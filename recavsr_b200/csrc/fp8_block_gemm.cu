@@ -690,10 +690,10 @@ __device__ __forceinline__ void store_piece(const Params& p, int row, int n, con
 }
 
 // ---------------------------------------------------------------- few rows
-// The same products with the operands' roles exchanged, for outputs of too few
-// 128 x 128 tiles to fill the GPU: W's 128 rows are the MMA's M side and the
-// BT (16 or 32) rows of A its N side, so a single row of A costs a 16-column
-// MMA; and a cluster of up to 8 CTAs splits K. Each CTA accumulates its k-tiles
+// The same products with the operands' roles exchanged, for up to 32 rows: W's
+// 128 rows are the MMA's M side and all rows of A (BT = 16 or 32 with the zeros
+// that fill them up) its N side, so a single row of A costs a 16-column MMA; and
+// a cluster of up to 8 CTAs splits K. Each CTA accumulates its k-tiles
 // in TMEM and pushes its fp32 partial, row of A by row, into the shared memory
 // of the CTA that owns the row (stores do not wait for the other SM, reads
 // would); after a cluster barrier each CTA sums its rows' partials in rank
@@ -735,8 +735,7 @@ rows_kernel(const __grid_constant__ Maps maps, const Params p, int split) {
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)sm100::cluster_ctarank();
-  const int tile = blockIdx.x / split;
-  const int tt = tile % p.m_blocks, wt = tile / p.m_blocks;     // tiles of one W block are neighbours
+  const int wt = blockIdx.x / split;                            // W's block of 128 rows, or of 128 gate and 128 up rows
   const int kt0 = (int)((long long)rank * p.k_tiles / split), kt1 = (int)((long long)(rank + 1) * p.k_tiles / split);
 
   if (threadIdx.x == 0) {
@@ -782,12 +781,12 @@ rows_kernel(const __grid_constant__ Maps maps, const Params p, int split) {
 #pragma unroll
         for (int w = 0; w < kW; ++w)
           sm100::tma_load_2d(a + w * BM * kRowBytes, &maps.b, &full[stage], kt * kRowBytes, (wt * kW + w) * BM);
-        sm100::tma_load_2d(a + kW * BM * kRowBytes, &maps.a, &full[stage], kt * kRowBytes, tt * BT);
+        sm100::tma_load_2d(a + kW * BM * kRowBytes, &maps.a, &full[stage], kt * kRowBytes, 0);
         if (atom) {
 #pragma unroll
           for (int w = 0; w < kW; ++w)
             sm100::tma_load_2d(sf + w * kSfAtom, &maps.sfb, &full[stage], 0, (wt * kW + w) * p.katoms * 4 + line);
-          sm100::tma_load_2d(sf + kW * kSfAtom, &maps.sfa, &full[stage], 0, tt * BT / 128 * p.katoms * 4 + line);
+          sm100::tma_load_2d(sf + kW * kSfAtom, &maps.sfa, &full[stage], 0, line);
         }
         ++issued;
         if (++stage == STAGES) { stage = 0; phase ^= 1; }
@@ -831,7 +830,7 @@ rows_kernel(const __grid_constant__ Maps maps, const Params p, int split) {
     }
   }
   __syncwarp();
-  const int rows = min(BT, p.M - tt * BT), per = (rows + split - 1) / split;   // rank q owns rows q * per ...
+  const int rows = p.M, per = (rows + split - 1) / split;       // at most BT; rank q owns rows q * per ...
   float* part = reinterpret_cast<float*>(smem + S::offPart);    // [rank][kW][per][128]
   bool ok = true;
   if (warp >= 2) {
@@ -901,7 +900,7 @@ rows_kernel(const __grid_constant__ Maps maps, const Params p, int split) {
     const int n = wt * BM + lane * 4;
     if constexpr (EPI == EPI_OUT) {
 #pragma unroll
-      for (int j = 0; j < kRows; ++j) load_piece<Out>(p, tt * BT + first + min(i + j, mine - 1), n, near[j]);
+      for (int j = 0; j < kRows; ++j) load_piece<Out>(p, first + min(i + j, mine - 1), n, near[j]);
     }
     for (int q = 0; q < split; ++q) {
 #pragma unroll
@@ -919,7 +918,7 @@ rows_kernel(const __grid_constant__ Maps maps, const Params p, int split) {
 #pragma unroll
     for (int j = 0; j < kRows; ++j) {
       if (i + j >= mine) break;
-      const int row = tt * BT + first + i + j;
+      const int row = first + i + j;
 #pragma unroll
       for (int w = 0; w < kW; ++w) {
         v[j][w].x += bias[w].x;
@@ -952,11 +951,11 @@ rows_kernel(const __grid_constant__ Maps maps, const Params p, int split) {
     }
   }
   if constexpr (EPI == EPI_SWIGLU) {
-    // Zero scales: rows past M of this tile's 128 (or BT, the only tile), and
-    // the last block's neighbours up to the atom.
-    const int atoms = fp8b::atoms_of(p.H), last = (p.M + 127) / 128 * 128;
+    // Zero scales: rows past M of the atom's 128, and the last block's neighbours
+    // up to the atom.
+    const int atoms = fp8b::atoms_of(p.H);
     if (rank == 0)
-      for (int row = tt * 128 + threadIdx.x; row < min(tt * 128 + 128, last); row += kRowsThreads) {
+      for (int row = threadIdx.x; row < 128; row += kRowsThreads) {
         if (row >= p.M) p.scales[rc::sf_offset(row, wt, atoms)] = 0;
         if (wt == p.n_blocks - 1)
           for (int kb = p.n_blocks; kb < 4 * atoms; ++kb) p.scales[rc::sf_offset(row, kb, atoms)] = 0;
@@ -970,7 +969,7 @@ int launch_rows(const Maps& maps, const Params& p, int split, cudaStream_t strea
   auto kern = rows_kernel<BT, EPI, Out>;
   static rc::SmemAttrFlags flags = {};
   if (const int r = rc::ensure_smem_attr(flags, reinterpret_cast<const void*>(kern), S::kTotal, what)) return r;
-  return rc::check_launch(rc::launch_pdl_cluster(kern, dim3((unsigned)(p.m_blocks * p.n_blocks * split)),
+  return rc::check_launch(rc::launch_pdl_cluster(kern, dim3((unsigned)(p.n_blocks * split)),
                                                  dim3(kRowsThreads), S::kTotal, stream, (unsigned)split, maps, p, split),
                           what);
 }
