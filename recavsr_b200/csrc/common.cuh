@@ -117,6 +117,27 @@ inline cudaError_t launch_pdl_cluster(void (*kernel)(KArgs...), dim3 grid, dim3 
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
+// Clusters of cluster_x CTAs that the current device runs at once; 0 where it
+// cannot tell.
+template <typename... KArgs>
+inline int resident_clusters(void (*kernel)(KArgs...), dim3 block, size_t smem, unsigned cluster_x) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(cluster_x);
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster_x;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) == cudaSuccess) return n;
+  cudaGetLastError();
+  return 0;
+}
+
 // Launch `kernel` on `stream` with programmatic stream serialization allowed.
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,

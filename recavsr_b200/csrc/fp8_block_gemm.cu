@@ -28,6 +28,8 @@
 // that the MMAs take from L2, then the power cap; at short K the hand-over of
 // the 256-column accumulator (a tile of CTA pairs at K = 512 takes 3100-3700
 // cycles, 2048 of them MMAs) and, gated, two MUFU results per output.
+#include <atomic>
+
 #include "fp8_block.cuh"
 #include "sm100.cuh"
 
@@ -702,7 +704,7 @@ __device__ __forceinline__ void store_piece(const Params& p, int row, int n, con
 // side by side (kW = 2): a row's 128 outputs are one warp's, so the block's
 // amax is one warp reduction. Measured: 1 x 3072 x 3072 4.0 us (2.35 TB/s of
 // weight), 24 x 3072 x 14336 11.0 us (4.1 TB/s), 1 x 512 x 512 2.8 us; bound by
-// the launch and the round trips before and after a CTA's 4 to 14 k-tiles.
+// the launch and the round trips before and after a CTA's k-tiles (4, 14 and 1 here).
 constexpr int kRowsThreads = 192;     // producer, MMA issuer, 4 TMEM warps; all 6 in the epilogue
 
 template <int BT, int EPI>
@@ -710,7 +712,7 @@ struct RowsSmem {
   static constexpr int kW = EPI == EPI_SWIGLU ? 2 : 1;
   static constexpr int kStage = (kW * BM + BT) * kRowBytes;
   static constexpr int kSf = (kW + 1) * kSfAtom;
-  static constexpr int kStages = 98304 / (kStage + kSf);    // two CTAs per SM where they fit
+  static constexpr int kStages = 98304 / (kStage + kSf);    // two CTAs per SM, but for gated tiles of 32 rows
   static constexpr int kPart = kW * (BT + 8) * BM * 4;      // the partials of the rows this CTA owns, by rank
   static constexpr int offPart = kStages * kStage;
   static constexpr int offSf = offPart + kPart;
@@ -718,6 +720,7 @@ struct RowsSmem {
   static constexpr int kTotal = offBar + (2 * kStages + 3) * 8;
   static constexpr int kTmem = kW * BT + 2 * 4 * (kW + 1);
   static constexpr int kTmemCols = kTmem <= 32 ? 32 : kTmem <= 64 ? 64 : kTmem <= 128 ? 128 : kTmem <= 256 ? 256 : 512;
+  static constexpr int kPerSm = 2 * (kTotal + 1024) <= 233472 ? 2 : 1;    // of 228 KB an SM, 1 KB kept for each CTA
   static_assert(kTotal <= 232448, "shared memory");
 };
 
@@ -963,12 +966,44 @@ rows_kernel(const __grid_constant__ Maps maps, const Params p, int split) {
   }
 }
 
+// CTAs of a cluster along K: as many as every cluster of the launch finds room
+// with at once, up to 8 and the k-tiles; one cluster too many is a second wave. A
+// cluster stays within one group of SMs, so the room is less than the SMs', and
+// the driver knows it for one CTA on each (clusters of 2 to 8 on a B200: 74, 45,
+// 33, 26, 22, 15, 15). Gated tiles of 32 rows are alone on their SM. The others
+// run two to an SM: twice the room, and clusters of 6 and 8 at least as many as
+// of 3 and 4 (measured: 45 of 45, 33 of 33; of 4 not as many as of 2, 71 of 74).
+// Measured (us) beside two CTAs for every SM: gated 32 x 8192 x 512 5.8 (10.4), 32
+// x 2048 x 4096 6.9 (11.9), 16 x 4736 x 4096 11.4 (16.3), 1 x 6144 x 3072 5.3 (8.0).
 template <int BT, int EPI, typename Out>
-int launch_rows(const Maps& maps, const Params& p, int split, cudaStream_t stream, const char* what) {
+int rows_split(const Params& p) {
+  using S = RowsSmem<BT, EPI>;
+  static std::atomic<int> cache[rc::kMaxDevices][9] = {};    // clusters + 1, 0: not asked yet
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= rc::kMaxDevices) return 1;
+  auto clusters = [&](int size) {
+    int n = cache[dev][size].load(std::memory_order_relaxed) - 1;
+    if (n < 0) {
+      n = rc::resident_clusters(rows_kernel<BT, EPI, Out>, dim3(kRowsThreads), S::kTotal, (unsigned)size);
+      cache[dev][size].store(n + 1, std::memory_order_relaxed);
+    }
+    return n;
+  };
+  for (int split = p.k_tiles < 8 ? p.k_tiles : 8; split > 1; --split) {
+    int room = S::kPerSm * clusters(split);
+    if (S::kPerSm == 2 && (split == 6 || split == 8) && room < clusters(split / 2)) room = clusters(split / 2);
+    if (p.n_blocks <= room) return split;
+  }
+  return 1;
+}
+
+template <int BT, int EPI, typename Out>
+int launch_rows(const Maps& maps, const Params& p, cudaStream_t stream, const char* what) {
   using S = RowsSmem<BT, EPI>;
   auto kern = rows_kernel<BT, EPI, Out>;
   static rc::SmemAttrFlags flags = {};
   if (const int r = rc::ensure_smem_attr(flags, reinterpret_cast<const void*>(kern), S::kTotal, what)) return r;
+  const int split = rows_split<BT, EPI, Out>(p);
   return rc::check_launch(rc::launch_pdl_cluster(kern, dim3((unsigned)(p.n_blocks * split)),
                                                  dim3(kRowsThreads), S::kTotal, stream, (unsigned)split, maps, p, split),
                           what);
@@ -1185,18 +1220,18 @@ bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0;
 // How a product runs.
 struct Plan {
   int bt;        // rows kernel with BT rows of A per tile; 0: tile kernel
-  int split;     // rows kernel, and split kernel (bt 0, split > 1): CTAs per tile along K
+  int split;     // split kernel (bt 0, split > 1): CTAs per tile along K
   int bn;        // tile kernel: columns per tile
   bool pair;     // tile kernel: CTA pairs (256-row tiles)
 };
 
-// Up to 32 rows run on the rows kernel, K split until two CTAs per SM have
-// work (measured, B200, us, split 1 / 2 / 4 / 8: 1 x 512 x 512 3.3 / 3.0 / 2.8
-// / -, 1 x 3072 x 3072 - / 4.9 / 4.1 / 4.2, 24 x 3072 x 14336 - / - / 14.0 /
-// 11.1; the tile kernel 4.1, 7.1 and 33). More rows take the tile kernel whose
-// waves cost least: cycles of a k-tile and of a tile's hand-over with every SM
-// busy, and of what comes before the first and after the last tile, fitted to
-// measurements. What they decide (us on 128 x 128 / pairs' 256 x 192 / 256 x
+// Up to 32 rows run on the rows kernel, which splits K itself (rows_split; us at
+// split 1 / 2 / 4 / 8: 1 x 512 x 512 3.2 / 2.8 / 2.6 / -, 1 x 3072 x 3072 6.7 / 4.9 /
+// 4.0 / 4.3, 24 x 3072 x 14336 - / - / 14.0 / 11.1; the tile kernel 4.1, 7.1 and
+// 33). More rows take the tile kernel whose waves cost least: cycles of a k-tile
+// and of a tile's hand-over with every SM busy, and of what comes before the first
+// and after the last tile, fitted to measurements. What they decide (with a
+// residual, us on 128 x 128 / pairs' 256 x 192 / 256 x
 // 256): 3520 x 768 x 512 6.1 / 6.5 / 7.3, 880 x 3072 x 3072 14.6 / 11.7 /
 // 13.9, 1759 x 3072 x 3072 22.1 / 18.3 / 22.0, 2500 x 4096 x 2048 27.0 / 21.6 /
 // 25.4, 300 x 9216 x 3072 17.1 / 18.3 / 15.5, 7040 x 3072 x 14336 318 / 250 /
@@ -1209,9 +1244,6 @@ Plan plan_for(int M, int N, int K, bool swiglu) {
   Plan q{0, 1, 256, false};
   if (M <= 32) {
     q.bt = M <= 16 ? 16 : 32;
-    const long long room = 2LL * sms / up(N, swiglu ? 256 : 128);
-    q.split = (int)(room < 1 ? 1 : room > 8 ? 8 : room);
-    if (q.split > k_tiles) q.split = k_tiles;
     return q;
   }
   struct Tile { int m, n, k_tile, tile, ends; };
@@ -1266,7 +1298,7 @@ int prepare(const char* what, const void* a, long long lda, const void* sa, cons
   p.inv_group = (uint32_t)((0x100000000ull + p.group_m - 1) / p.group_m);
   p.inv_last = (uint32_t)((0x100000000ull + last - 1) / last);
   const long long lines_a = 4LL * p.katoms * ((M + 127) / 128), lines_b = 4LL * p.katoms * ((N + 127) / 128);
-  if ((long long)p.m_blocks * p.n_blocks * q.split > INT32_MAX || p.n_blocks > (1 << 24) || lines_a > INT32_MAX || lines_b > INT32_MAX)
+  if ((long long)p.m_blocks * p.n_blocks * 8 > INT32_MAX || p.n_blocks > (1 << 24) || lines_a > INT32_MAX || lines_b > INT32_MAX)
     return rc::set_error(RC_ERR_UNSUPPORTED, "%s: %d x %d x %d is too large", what, M, N, K);
   const uint32_t box_a[2] = {kRowBytes, (uint32_t)rows_a}, box_b[2] = {kRowBytes, (uint32_t)rows_b}, box_s[2] = {128, 4};
   const uint64_t da[2] = {(uint64_t)K, (uint64_t)M}, db[2] = {(uint64_t)K, (uint64_t)N};
@@ -1301,8 +1333,8 @@ int check_operands(const char* what, const void* a, long long lda, const void* s
 
 template <int EPI, typename Out>
 int run(const Maps& maps, const Params& p, const Plan& q, cudaStream_t stream, const char* what) {
-  if (q.bt == 16) return launch_rows<16, EPI, Out>(maps, p, q.split, stream, what);
-  if (q.bt == 32) return launch_rows<32, EPI, Out>(maps, p, q.split, stream, what);
+  if (q.bt == 16) return launch_rows<16, EPI, Out>(maps, p, stream, what);
+  if (q.bt == 32) return launch_rows<32, EPI, Out>(maps, p, stream, what);
   if constexpr (EPI == EPI_OUT) {
     if (q.split == 2) return launch_split<2, Out>(maps, p, stream, what);
     if (q.split == 4) return launch_split<4, Out>(maps, p, stream, what);

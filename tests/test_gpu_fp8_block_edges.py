@@ -42,6 +42,38 @@ def test_few_rows_back_to_back(n, k):
     assert_no_device_error()
 
 
+def _microseconds(call, launches=20, times=7):
+    """Least device time of one launch out of a graph of them."""
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(launches):
+            call()
+    best = float("inf")
+    for _ in range(times):
+        begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        begin.record()
+        graph.replay()
+        end.record()
+        end.synchronize()
+        best = min(best, begin.elapsed_time(end) * 1e3 / launches)
+    return best
+
+
+@pytest.mark.parametrize("fits,more,k", [(4096, 8192, 512), (1792, 2048, 4096)])
+def test_few_rows_run_in_one_wave(fits, more, k):
+    """Gated tiles of 32 rows have an SM to themselves: more tiles than clusters
+    find room for must mean smaller clusters, not a second wave (twice the time)."""
+    from recavsr_b200.runtime import fp8_block
+    took = []
+    for h in (fits, more):
+        ac, asc = fp8_block.quantize(activations(32, k, torch.bfloat16, 51))
+        wc, wsc = fp8_block.quantize_weight(torch.randn(2 * h, k, device="cuda") / k ** 0.5)
+        took.append(_microseconds(lambda: fp8_block.swiglu_mm(ac, wc, asc, wsc)))
+    assert took[1] < 1.5 * took[0], took
+
+
 # ---------------------------------------------------------------- gates far from zero
 # Instruction errors of silu(g) u = g / (1 + t) * p * u * p with t = s^2 = exp(-|g|) and p = s below zero, else 1:
 # s carries 2^-22 of the exponential and |g| / 2 (2^-24 + 2^-26) of its rounded argument, both twice in p p and once
