@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import argparse
 import concurrent.futures as cf
+import importlib.metadata
 import os
 import shutil
 import subprocess
@@ -23,6 +24,7 @@ CSRC = os.path.join(PKG, "csrc")
 OBJ = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "librecavsr_b200.so")
 BINDING = os.path.join(PKG, "_fp8_block.so")
+BINDING_KEY = os.path.join(OBJ, "_fp8_block.key")
 BINDING_SOURCE = os.path.join(CSRC, "fp8_block_torch.cpp")
 INCLUDE = os.path.join(os.path.dirname(PKG), "include", "recavsr_b200.h")
 SOURCES = ["runtime.cu", "quant.cu", "glue.cu", "gemm.cu", "attention.cu", "session.cu", "pipeline.cu", "decoder_attention.cu", "decoder.cu", "colorfix.cu",
@@ -58,8 +60,19 @@ def _compile(src: str, force: bool) -> str:
     return obj
 
 
+def _binding_key() -> str:
+    """What the binding's object layouts depend on besides its own sources."""
+    return f"torch {importlib.metadata.version('torch')}, {sysconfig.get_config_var('SOABI')}"
+
+
 def _build_binding(force: bool) -> None:
-    if not force and not _stale(BINDING, [BINDING_SOURCE, INCLUDE]):
+    try:
+        with open(BINDING_KEY) as f:
+            built_for = f.read()
+    except OSError:
+        built_for = None
+    key = _binding_key()
+    if not force and built_for == key and not _stale(BINDING, [BINDING_SOURCE, INCLUDE]):
         return
     import torch
 
@@ -67,15 +80,19 @@ def _build_binding(force: bool) -> None:
     cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc()))), "include")
     include = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
                sysconfig.get_paths()["include"], cuda]
+    part = BINDING + ".part"          # whole before it has its name: another process may be importing
     # The host compiler that nvcc uses, not $CXX: one with a C++ runtime of its
     # own linked in clashes with the runtime torch has loaded.
     cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{d}" for d in include),
-           BINDING_SOURCE, "-o", BINDING, "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu",
+           BINDING_SOURCE, "-o", part, "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu",
            "-ltorch_cuda", "-lc10", "-lc10_cuda", "-L" + PKG, "-l:" + os.path.basename(LIB), "-Wl,-rpath,$ORIGIN"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode:
         raise RuntimeError(f"{cmd[0]} failed for {os.path.basename(BINDING_SOURCE)}:\n{r.stderr}")
+    os.replace(part, BINDING)
+    with open(BINDING_KEY, "w") as f:
+        f.write(key)
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
