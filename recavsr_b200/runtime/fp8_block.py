@@ -15,7 +15,8 @@ weights one for each 128 x 128 block.
     codes, scales = swiglu_mm(codes, gu_codes, scales, gu_scales, gu_bias)
 
 Every function runs on the current stream of its inputs' device and allocates
-only what it returns. There is no CPU path.
+only what it returns. There is no CPU path. A call goes straight to the binding;
+under torch.compile it goes through a custom op.
 """
 from __future__ import annotations
 
@@ -74,6 +75,10 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float, residua
     without a residual) and the norm h * rsqrt(mean(h^2) + eps) * weight is
     quantized from fp32, without a rounding between. Rows of at most 16384
     columns, a multiple of 16."""
+    if torch.compiler.is_compiling():
+        if residual is None:
+            return (*torch.ops.recavsr_b200.fp8_block_rms_norm(x, weight, eps), None)
+        return torch.ops.recavsr_b200.fp8_block_add_rms_norm(x, weight, eps, residual)
     return _binding.rms_norm_quantize(x, weight, eps, residual)
 
 
@@ -83,9 +88,12 @@ def mm(values: torch.Tensor, weights: torch.Tensor, scales: torch.Tensor, weight
     """[M, N] = A [M, K] . W [N, K]^T + bias (+ residual), summed in fp32 and
     rounded once to dtype (bfloat16 by default, or float16; the residual has the
     same). `out` may be `residual` itself."""
-    if torch.compiler.is_compiling() and out is None:
+    if not torch.compiler.is_compiling():
+        return _binding.mm(values, weights, scales, weight_scales, bias, residual, dtype, out)
+    if out is None:
         return torch.ops.recavsr_b200.fp8_block_mm(values, weights, scales, weight_scales, bias, residual, dtype)
-    return _binding.mm(values, weights, scales, weight_scales, bias, residual, dtype, out)
+    torch.ops.recavsr_b200.fp8_block_mm_out(values, weights, scales, weight_scales, bias, residual, dtype, out)
+    return out
 
 
 def interleave_gate_up(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
@@ -106,6 +114,8 @@ def swiglu_mm(values: torch.Tensor, weights: torch.Tensor, scales: torch.Tensor,
     """silu(A . Wg^T + bg) * (A . Wu^T + bu) held in 8 bits: (codes, scales) of
     [M, features]. weights and bias come in interleave_gate_up's order;
     features (a multiple of 16) defaults to half the weight's rows."""
+    if torch.compiler.is_compiling():
+        return torch.ops.recavsr_b200.fp8_block_swiglu_mm(values, weights, scales, weight_scales, bias, features)
     return _binding.swiglu_mm(values, weights, scales, weight_scales, bias, features)
 
 
@@ -120,6 +130,27 @@ def _quantize_fake(x, weight):
             x.new_empty((scale_numel(*x.shape),), dtype=torch.uint8))
 
 
+@torch.library.custom_op("recavsr_b200::fp8_block_rms_norm", mutates_args=())
+def _rms_norm_op(x: torch.Tensor, weight: torch.Tensor, eps: float) -> tuple[torch.Tensor, torch.Tensor]:
+    return _binding.rms_norm_quantize(x, weight, eps, None)[:2]
+
+
+@_rms_norm_op.register_fake
+def _rms_norm_fake(x, weight, eps):
+    return _quantize_fake(x, False)
+
+
+@torch.library.custom_op("recavsr_b200::fp8_block_add_rms_norm", mutates_args=())
+def _add_rms_norm_op(x: torch.Tensor, weight: torch.Tensor, eps: float,
+                     residual: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _binding.rms_norm_quantize(x, weight, eps, residual)
+
+
+@_add_rms_norm_op.register_fake
+def _add_rms_norm_fake(x, weight, eps, residual):
+    return (*_quantize_fake(x, False), x.new_empty(x.shape))
+
+
 @torch.library.custom_op("recavsr_b200::fp8_block_mm", mutates_args=())
 def _mm_op(values: torch.Tensor, weights: torch.Tensor, scales: torch.Tensor, weight_scales: torch.Tensor,
            bias: torch.Tensor | None, residual: torch.Tensor | None, dtype: torch.dtype | None) -> torch.Tensor:
@@ -130,6 +161,31 @@ def _mm_op(values: torch.Tensor, weights: torch.Tensor, scales: torch.Tensor, we
 def _mm_fake(values, weights, scales, weight_scales, bias, residual, dtype):
     dtype = dtype or (torch.bfloat16 if residual is None else residual.dtype)
     return values.new_empty((values.shape[0], weights.shape[0]), dtype=dtype)
+
+
+@torch.library.custom_op("recavsr_b200::fp8_block_mm_out", mutates_args=("out",))
+def _mm_out_op(values: torch.Tensor, weights: torch.Tensor, scales: torch.Tensor, weight_scales: torch.Tensor,
+               bias: torch.Tensor | None, residual: torch.Tensor | None, dtype: torch.dtype | None,
+               out: torch.Tensor) -> None:
+    _binding.mm(values, weights, scales, weight_scales, bias, residual, dtype, out)
+
+
+@_mm_out_op.register_fake
+def _mm_out_fake(values, weights, scales, weight_scales, bias, residual, dtype, out):
+    return None
+
+
+@torch.library.custom_op("recavsr_b200::fp8_block_swiglu_mm", mutates_args=())
+def _swiglu_mm_op(values: torch.Tensor, weights: torch.Tensor, scales: torch.Tensor, weight_scales: torch.Tensor,
+                  bias: torch.Tensor | None, features: int | None) -> tuple[torch.Tensor, torch.Tensor]:
+    return _binding.swiglu_mm(values, weights, scales, weight_scales, bias, features)
+
+
+@_swiglu_mm_op.register_fake
+def _swiglu_mm_fake(values, weights, scales, weight_scales, bias, features):
+    rows, h = values.shape[0], weights.shape[0] // 2 if features is None else features
+    return (values.new_empty((rows, h), dtype=torch.uint8),
+            values.new_empty((scale_numel(rows, h),), dtype=torch.uint8))
 
 
 class BlockFP8Linear(nn.Module):

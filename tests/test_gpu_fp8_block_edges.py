@@ -153,3 +153,31 @@ def test_swiglu_strided_codes(m):
         wide[:, at:at + 256], weight[:, at:at + 256] = ac, wc
         got = fp8_block.swiglu_mm(wide[:, at:at + 256], weight[:, at:at + 256], asc, wsc)
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ---------------------------------------------------------------- torch.compile
+@pytest.mark.parametrize("dynamic", [False, True])
+def test_operators_compile(dynamic):
+    """torch.compile(fullgraph=True) traces through all four, in-place products among them."""
+    from recavsr_b200.runtime import fp8_block
+    w = torch.ones(512, device="cuda")
+    wo = fp8_block.quantize_weight(activations(512, 512, torch.bfloat16, 63))
+    gu = fp8_block.quantize_weight(fp8_block.interleave_gate_up(*activations(416, 512, torch.bfloat16, 64).chunk(2)))
+    down = fp8_block.quantize_weight(activations(512, 208, torch.bfloat16, 65))
+    bias = torch.randn(512, device="cuda", generator=torch.Generator("cuda").manual_seed(66))
+
+    def block(x, hidden):
+        codes, scales, _ = fp8_block.rms_norm_quantize(x, w, 1e-5)
+        delta = fp8_block.mm(codes, wo[0], scales, wo[1], bias)
+        codes, scales, hidden = fp8_block.rms_norm_quantize(delta, w, 1e-5, residual=hidden)
+        codes, scales = fp8_block.swiglu_mm(codes, gu[0], scales, gu[1], features=208)
+        out = hidden.clone()
+        fp8_block.mm(codes, down[0], scales, down[1], bias, residual=out, out=out)
+        return out, codes, scales
+
+    compiled = torch.compile(block, fullgraph=True, backend="aot_eager", dynamic=dynamic)
+    with torch.inference_mode():
+        for rows in (37, 300):
+            x, r = activations(rows, 512, torch.bfloat16, rows), activations(rows, 512, torch.bfloat16, rows + 1)
+            for got, want in zip(compiled(x, r), block(x, r)):
+                assert torch.equal(got, want)
