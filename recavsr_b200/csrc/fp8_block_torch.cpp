@@ -7,6 +7,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -104,6 +105,10 @@ PyObject* pair(const at::Tensor& a, const at::Tensor& b) {
   return t;
 }
 
+// A gradient would be asked for: the caller takes the call through a custom op,
+// whose result raises in backward.
+bool wants_grad(const at::Tensor& t) { return t.defined() && t.requires_grad() && c10::GradMode::is_enabled(); }
+
 #define EXPECT_ARGS(count) TORCH_CHECK(nargs == (count), "expected ", (count), " arguments (got ", nargs, ")")
 
 // quantize(x, what, weight) -> (codes, scales)
@@ -123,7 +128,7 @@ PyObject* quantize(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-// rms_norm_quantize(x, weight, eps, residual | None) -> (codes, scales, hidden | None)
+// rms_norm_quantize(x, weight, eps, residual | None) -> (codes, scales, hidden | None) or NotImplemented (wants_grad)
 PyObject* rms_norm_quantize(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   EXPECT_ARGS(4);
@@ -139,6 +144,7 @@ PyObject* rms_norm_quantize(PyObject*, PyObject* const* args, Py_ssize_t nargs) 
     const at::Tensor& r = tensor(args[3], what, "residual");
     TORCH_CHECK_VALUE(r.sizes() == x.sizes() && r.scalar_type() == x.scalar_type() && r.device() == x.device(), what,
                       ": residual must match x's shape, dtype and device.");
+    if (wants_grad(x) || wants_grad(r)) return Py_NewRef(Py_NotImplemented);
     residual = rows(r, what);
     hidden = empty({m, n}, x.scalar_type(), x);
   }
@@ -159,7 +165,8 @@ PyObject* rms_norm_quantize(PyObject*, PyObject* const* args, Py_ssize_t nargs) 
   END_HANDLE_TH_ERRORS
 }
 
-// mm(values, weights, scales, weight_scales, bias, residual, dtype, out), the last four or None
+// mm(values, weights, scales, weight_scales, bias, residual, dtype, out), the last four or None; -> out or NotImplemented
+// (wants_grad)
 PyObject* mm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   EXPECT_ARGS(8);
@@ -183,11 +190,13 @@ PyObject* mm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   c10::cuda::CUDAGuard guard(a.device());
   at::Tensor bias, residual, out;
   if (args[4] != Py_None) bias = vector(tensor(args[4], what, "bias"), n, a, "fp8_block.mm: bias");
+  bool grad = wants_grad(bias);
   if (args[5] != Py_None) {
     residual = tensor(args[5], what, "residual");
     TORCH_CHECK_VALUE(residual.dim() == 2 && residual.size(0) == m && residual.size(1) == n &&
                           residual.scalar_type() == dtype && residual.device() == a.device(),
                       what, ": residual must be ", m, " x ", n, " ", dtype, " on ", a.device(), ".");
+    grad |= wants_grad(residual);
     if (!is_rows(residual)) residual = residual.clone(at::MemoryFormat::Contiguous);
   }
   if (args[7] != Py_None) {
@@ -195,9 +204,10 @@ PyObject* mm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     TORCH_CHECK_VALUE(out.dim() == 2 && out.size(0) == m && out.size(1) == n && out.scalar_type() == dtype &&
                           out.device() == a.device() && is_rows(out),
                       what, ": out must be ", m, " x ", n, " ", dtype, " rows on ", a.device(), ".");
-  } else {
-    out = empty({m, n}, dtype, a);
+    grad |= wants_grad(out);
   }
+  if (grad) return Py_NewRef(Py_NotImplemented);
+  if (!out.defined()) out = empty({m, n}, dtype, a);
   check(rc_fp8_block_gemm(bytes(a), row_stride(a), bytes(scales), bytes(b), row_stride(b), bytes(weight_scales),
                           bias.defined() ? static_cast<const float*>(bias.const_data_ptr()) : nullptr, m, n, k,
                           dtype_code(dtype), residual.defined() ? residual.const_data_ptr() : nullptr,

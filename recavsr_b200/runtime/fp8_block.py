@@ -15,8 +15,12 @@ weights one for each 128 x 128 block.
     codes, scales = swiglu_mm(codes, gu_codes, scales, gu_scales, gu_bias)
 
 Every function runs on the current stream of its inputs' device and allocates
-only what it returns. There is no CPU path. A call goes straight to the binding;
-under torch.compile it goes through a custom op.
+only what it returns. There is no CPU path. None has a backward pass: codes carry
+no gradient, and a floating-point result of inputs that require one raises in
+backward (mm into `out` refuses such inputs, as torch's functions do).
+
+A call goes straight to the binding; under torch.compile, or where a gradient
+would be asked for (the binding answers NotImplemented), through a custom op.
 """
 from __future__ import annotations
 
@@ -79,7 +83,10 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float, residua
         if residual is None:
             return (*torch.ops.recavsr_b200.fp8_block_rms_norm(x, weight, eps), None)
         return torch.ops.recavsr_b200.fp8_block_add_rms_norm(x, weight, eps, residual)
-    return _binding.rms_norm_quantize(x, weight, eps, residual)
+    result = _binding.rms_norm_quantize(x, weight, eps, residual)
+    if result is NotImplemented:
+        return torch.ops.recavsr_b200.fp8_block_add_rms_norm(x, weight, eps, residual)
+    return result
 
 
 def mm(values: torch.Tensor, weights: torch.Tensor, scales: torch.Tensor, weight_scales: torch.Tensor,
@@ -88,10 +95,15 @@ def mm(values: torch.Tensor, weights: torch.Tensor, scales: torch.Tensor, weight
     """[M, N] = A [M, K] . W [N, K]^T + bias (+ residual), summed in fp32 and
     rounded once to dtype (bfloat16 by default, or float16; the residual has the
     same). `out` may be `residual` itself."""
+    result = NotImplemented
     if not torch.compiler.is_compiling():
-        return _binding.mm(values, weights, scales, weight_scales, bias, residual, dtype, out)
+        result = _binding.mm(values, weights, scales, weight_scales, bias, residual, dtype, out)
+    if result is not NotImplemented:
+        return result
     if out is None:
         return torch.ops.recavsr_b200.fp8_block_mm(values, weights, scales, weight_scales, bias, residual, dtype)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (bias, residual, out)):
+        raise ValueError("fp8_block.mm: with out there is no gradient, but an argument requires one.")
     torch.ops.recavsr_b200.fp8_block_mm_out(values, weights, scales, weight_scales, bias, residual, dtype, out)
     return out
 
@@ -143,7 +155,8 @@ def _rms_norm_fake(x, weight, eps):
 @torch.library.custom_op("recavsr_b200::fp8_block_add_rms_norm", mutates_args=())
 def _add_rms_norm_op(x: torch.Tensor, weight: torch.Tensor, eps: float,
                      residual: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    return _binding.rms_norm_quantize(x, weight, eps, residual)
+    with torch.no_grad():
+        return _binding.rms_norm_quantize(x, weight, eps, residual)
 
 
 @_add_rms_norm_op.register_fake
@@ -154,7 +167,8 @@ def _add_rms_norm_fake(x, weight, eps, residual):
 @torch.library.custom_op("recavsr_b200::fp8_block_mm", mutates_args=())
 def _mm_op(values: torch.Tensor, weights: torch.Tensor, scales: torch.Tensor, weight_scales: torch.Tensor,
            bias: torch.Tensor | None, residual: torch.Tensor | None, dtype: torch.dtype | None) -> torch.Tensor:
-    return _binding.mm(values, weights, scales, weight_scales, bias, residual, dtype, None)
+    with torch.no_grad():
+        return _binding.mm(values, weights, scales, weight_scales, bias, residual, dtype, None)
 
 
 @_mm_op.register_fake
@@ -167,7 +181,8 @@ def _mm_fake(values, weights, scales, weight_scales, bias, residual, dtype):
 def _mm_out_op(values: torch.Tensor, weights: torch.Tensor, scales: torch.Tensor, weight_scales: torch.Tensor,
                bias: torch.Tensor | None, residual: torch.Tensor | None, dtype: torch.dtype | None,
                out: torch.Tensor) -> None:
-    _binding.mm(values, weights, scales, weight_scales, bias, residual, dtype, out)
+    with torch.no_grad():
+        _binding.mm(values, weights, scales, weight_scales, bias, residual, dtype, out)
 
 
 @_mm_out_op.register_fake
@@ -186,6 +201,19 @@ def _swiglu_mm_fake(values, weights, scales, weight_scales, bias, features):
     rows, h = values.shape[0], weights.shape[0] // 2 if features is None else features
     return (values.new_empty((rows, h), dtype=torch.uint8),
             values.new_empty((scale_numel(rows, h),), dtype=torch.uint8))
+
+
+@torch.library.custom_op("recavsr_b200::fp8_block_linear", mutates_args=())
+def _linear_op(x: torch.Tensor, weights: torch.Tensor, weight_scales: torch.Tensor,
+               bias: torch.Tensor | None) -> torch.Tensor:
+    with torch.no_grad():
+        codes, scales = _binding.quantize(x, False)
+        return _binding.mm(codes, weights, scales, weight_scales, bias, None, x.dtype, None)
+
+
+@_linear_op.register_fake
+def _linear_fake(x, weights, weight_scales, bias):
+    return x.new_empty((x.shape[0], weights.shape[0]))
 
 
 class BlockFP8Linear(nn.Module):
@@ -208,8 +236,12 @@ class BlockFP8Linear(nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if x.dtype not in (torch.bfloat16, torch.float16):
             raise ValueError("Block FP8 linears take BF16 or FP16 inputs and produce the same type.")
-        codes, scales = quantize(x.reshape(-1, self.in_features))
-        out = mm(codes, self.weight_codes, scales, self.weight_scales, self.bias, dtype=x.dtype)
+        rows = x.reshape(-1, self.in_features)
+        if x.requires_grad and torch.is_grad_enabled():      # codes carry none: the op spans both steps
+            out = torch.ops.recavsr_b200.fp8_block_linear(rows, self.weight_codes, self.weight_scales, self.bias)
+        else:
+            codes, scales = quantize(rows)
+            out = mm(codes, self.weight_codes, scales, self.weight_scales, self.bias, dtype=x.dtype)
         return out.reshape(*x.shape[:-1], self.out_features)
 
 

@@ -155,7 +155,40 @@ def test_swiglu_strided_codes(m):
         assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
-# ---------------------------------------------------------------- torch.compile
+# ---------------------------------------------------------------- gradients and torch.compile
+def test_lost_gradients_raise():
+    """No operator has a backward pass: a result whose gradient would be asked for
+    says so in backward instead of standing there as a constant."""
+    from recavsr_b200.runtime import fp8_block
+    x, w = activations(5, 128, torch.bfloat16, 61), torch.ones(128, device="cuda")
+    (ac, asc), (bc, bsc) = fp8_block.quantize(x), fp8_block.quantize_weight(activations(64, 128, torch.bfloat16, 62))
+    bias, res = torch.zeros(64, device="cuda"), torch.zeros(5, 64, dtype=torch.bfloat16, device="cuda")
+    leaf = lambda t: t.clone().requires_grad_()
+    lin = fp8_block.BlockFP8Linear(torch.nn.Linear(128, 64, device="cuda", dtype=torch.bfloat16))
+    calls = [(lambda: fp8_block.mm(ac, bc, asc, bsc, leaf(bias)), lambda: fp8_block.mm(ac, bc, asc, bsc, bias)),
+             (lambda: fp8_block.mm(ac, bc, asc, bsc, residual=leaf(res)),
+              lambda: fp8_block.mm(ac, bc, asc, bsc, residual=res)),
+             (lambda: fp8_block.rms_norm_quantize(leaf(x), w, 1e-5, residual=x)[2],
+              lambda: fp8_block.rms_norm_quantize(x, w, 1e-5, residual=x)[2]),
+             (lambda: lin(leaf(x)), lambda: lin(x))]
+    for call, plain in calls:
+        got, want = call(), plain()
+        assert torch.equal(got, want) and got.requires_grad and not want.requires_grad
+        with pytest.raises(RuntimeError, match="no autograd formula"):
+            got.float().sum().backward()
+        with torch.no_grad():
+            assert not call().requires_grad
+    with pytest.raises(ValueError, match="gradient"):
+        fp8_block.mm(ac, bc, asc, bsc, leaf(bias), out=res)
+    with torch.no_grad():
+        assert fp8_block.mm(ac, bc, asc, bsc, leaf(bias), out=res) is not None
+    # codes are whole numbers: no gradient, and none promised
+    gu = fp8_block.quantize_weight(activations(256, 128, torch.bfloat16, 67))
+    for q in (fp8_block.quantize(leaf(x)), fp8_block.rms_norm_quantize(leaf(x), w, 1e-5)[:2],
+              fp8_block.swiglu_mm(ac, gu[0], asc, gu[1], leaf(torch.zeros(256, device="cuda")))):
+        assert not any(t.requires_grad for t in q)
+
+
 @pytest.mark.parametrize("dynamic", [False, True])
 def test_operators_compile(dynamic):
     """torch.compile(fullgraph=True) traces through all four, in-place products among them."""
