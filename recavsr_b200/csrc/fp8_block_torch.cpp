@@ -73,8 +73,11 @@ at::Tensor empty(at::IntArrayRef size, at::ScalarType type, const at::Tensor& li
 at::Tensor operand(const at::Tensor& codes, const at::Tensor& scales, const char* what) {
   TORCH_CHECK_VALUE(codes.is_cuda() && scales.device() == codes.device(), what,
                     ": codes and scales must be on one CUDA device (got ", codes.device(), ", ", scales.device(), ").");
-  TORCH_CHECK_VALUE(codes.dim() == 2 && codes.element_size() == 1 && scales.element_size() == 1, what,
-                    ": operands are 8-bit codes [rows, K] with 8-bit scales.");
+  // Other 8-bit types would be read as what they are not (a float8_e5m2 code as E4M3).
+  TORCH_CHECK_VALUE(codes.dim() == 2 && (codes.scalar_type() == at::kByte || codes.scalar_type() == at::kFloat8_e4m3fn) &&
+                        (scales.scalar_type() == at::kByte || scales.scalar_type() == at::kFloat8_e8m0fnu),
+                    what, ": operands are uint8 or float8_e4m3fn codes [rows, K] with uint8 or float8_e8m0fnu scales (got ",
+                    codes.dim(), "-D ", codes.scalar_type(), ", ", scales.scalar_type(), ").");
   const int64_t n = codes.size(0), k = codes.size(1);
   TORCH_CHECK_VALUE(k > 0 && k % 16 == 0, what, ": K must be a positive multiple of 16 (got ", k, ").");
   TORCH_CHECK_VALUE(n <= INT32_MAX && k <= INT32_MAX, what, ": ", n, " x ", k, " is too large.");

@@ -4,8 +4,8 @@ block of 128 columns, next to the per-tensor FP8 linears of runtime.fp8
 
 A matrix held in 8 bits is a pair (codes, scales): u8 E4M3 codes [rows, cols]
 and u8 E8M0 scale bytes (2^(e-127), the smallest with amax <= 448 * scale) in
-the flat 128x4 blocked order the tensor core reads; scale_bytes() gives them as
-[rows, blocks]. Activations have a scale for each row's block of 128 columns,
+the flat 128x4 blocked order the tensor core reads (as operands also in torch's
+float8_e4m3fn and float8_e8m0fnu); scale_bytes() gives them as [rows, blocks]. Activations have a scale for each row's block of 128 columns,
 weights one for each 128 x 128 block.
 
     codes, scales, hidden = rms_norm_quantize(x, weight, eps, residual=hidden)

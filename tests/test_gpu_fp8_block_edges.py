@@ -214,3 +214,21 @@ def test_operators_compile(dynamic):
             x, r = activations(rows, 512, torch.bfloat16, rows), activations(rows, 512, torch.bfloat16, rows + 1)
             for got, want in zip(compiled(x, r), block(x, r)):
                 assert torch.equal(got, want)
+
+
+# ---------------------------------------------------------------- refusals
+def test_other_eight_bit_types_are_refused():
+    """Bytes of another 8-bit format read as E4M3 codes or E8M0 scales would give wrong products."""
+    from recavsr_b200.runtime import fp8_block
+    a, s = fp8_block.quantize(activations(4, 256, torch.bfloat16, 71))
+    for t, ts in ((a.view(torch.float8_e4m3fn), s), (a, s.view(torch.float8_e8m0fnu))):
+        assert torch.equal(fp8_block.mm(t, a, ts, s), fp8_block.mm(a, a, s, s))
+    for dtype in (torch.float8_e5m2, torch.float8_e4m3fnuz, torch.int8, torch.bool):
+        for call in (lambda: fp8_block.mm(a.view(dtype), a, s, s), lambda: fp8_block.mm(a, a.view(dtype), s, s),
+                     lambda: fp8_block.swiglu_mm(a.view(dtype), a, s, s)):
+            with pytest.raises(ValueError, match="float8_e4m3fn codes"):
+                call()
+    for dtype in (torch.float8_e4m3fn, torch.int8):
+        for call in (lambda: fp8_block.mm(a, a, s.view(dtype), s), lambda: fp8_block.mm(a, a, s, s.view(dtype))):
+            with pytest.raises(ValueError, match="float8_e8m0fnu scales"):
+                call()
