@@ -87,6 +87,23 @@ at::Tensor operand(const at::Tensor& codes, const at::Tensor& scales, const char
   return codes.clone(at::MemoryFormat::Contiguous);
 }
 
+// Whether rows of two matrices share memory: [t.size(0), bytes] pieces every row
+// stride. Rows of one stride side by side (column ranges of one buffer) do not.
+bool share(const at::Tensor& a, const at::Tensor& b) {
+  if (!a.numel() || !b.numel()) return false;
+  const bool matrix = a.dim() == 2 && b.dim() == 2;
+  auto span = [](const at::Tensor& t) {
+    const int64_t last = t.dim() == 2 ? (t.size(0) - 1) * row_stride(t) + t.size(1) : t.numel();
+    return last * (int64_t)t.element_size();
+  };
+  const int64_t at = reinterpret_cast<int64_t>(a.const_data_ptr()), bt = reinterpret_cast<int64_t>(b.const_data_ptr());
+  if (at + span(a) <= bt || bt + span(b) <= at) return false;
+  const int64_t step = matrix ? row_stride(a) * (int64_t)a.element_size() : 0;
+  if (!matrix || step != row_stride(b) * (int64_t)b.element_size()) return true;
+  const int64_t from = ((bt - at) % step + step) % step;     // b's rows start here in a's
+  return from < a.size(1) * (int64_t)a.element_size() || from + b.size(1) * (int64_t)b.element_size() > step;
+}
+
 void check(int status) {
   if (!status) return;
   char text[1024];
@@ -208,6 +225,12 @@ PyObject* mm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
                           out.device() == a.device() && is_rows(out),
                       what, ": out must be ", m, " x ", n, " ", dtype, " rows on ", a.device(), ".");
     grad |= wants_grad(out);
+    // Tiles are written while others still read: out may be the residual, element for element, and no other input.
+    const bool same = residual.defined() && out.const_data_ptr() == residual.const_data_ptr() &&
+                      (row_stride(out) == row_stride(residual) || m == 1);
+    TORCH_CHECK_VALUE((!residual.defined() || same || !share(out, residual)) && !share(out, a) && !share(out, b) &&
+                          !share(out, scales) && !share(out, weight_scales) && (!bias.defined() || !share(out, bias)),
+                      what, ": out shares memory with an input (it may be the residual itself).");
   }
   if (grad) return Py_NewRef(Py_NotImplemented);
   if (!out.defined()) out = empty({m, n}, dtype, a);

@@ -94,7 +94,7 @@ def mm(values: torch.Tensor, weights: torch.Tensor, scales: torch.Tensor, weight
        dtype: torch.dtype | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """[M, N] = A [M, K] . W [N, K]^T + bias (+ residual), summed in fp32 and
     rounded once to dtype (bfloat16 by default, or float16; the residual has the
-    same). `out` may be `residual` itself."""
+    same). `out` may be `residual` itself; it shares memory with no other input."""
     result = NotImplemented
     if not torch.compiler.is_compiling():
         result = _binding.mm(values, weights, scales, weight_scales, bias, residual, dtype, out)

@@ -232,3 +232,39 @@ def test_other_eight_bit_types_are_refused():
         for call in (lambda: fp8_block.mm(a, a, s.view(dtype), s), lambda: fp8_block.mm(a, a, s, s.view(dtype))):
             with pytest.raises(ValueError, match="float8_e8m0fnu scales"):
                 call()
+
+
+@pytest.mark.parametrize("m", [1, 6, 200])
+def test_outputs_that_share_memory(m):
+    """out may be the residual, or lie beside any input in one buffer, but not over it."""
+    from recavsr_b200.runtime import fp8_block
+    n = k = 128
+    (ac, asc), (bc, bsc), _, _ = operands(m, n, k, 72)
+    buffer = activations(m + 2, 3 * n, torch.bfloat16, 73)
+    mm = lambda r, o, bias=None: fp8_block.mm(ac, bc, asc, bsc, bias, residual=r, out=o)
+    fresh = lambda: buffer.clone()
+    want = fp8_block.mm(ac, bc, asc, bsc, residual=buffer[:m, :n])
+    for at in (n, 2 * n):                        # columns beside the residual's
+        b = fresh()
+        assert torch.equal(mm(b[:m, :n], b[:m, at:at + n]), want)
+        assert torch.equal(b[:m, :n], buffer[:m, :n])
+    b = fresh()
+    assert torch.equal(mm(b[:m, :n], b[:m, :n]), want)
+    b = fresh()
+    for r, o in ((b[:m, :n], b[:m, 8:8 + n]), (b[:m, 8:8 + n], b[:m, :n]), (b[1:m + 1, :n], b[1:m + 1, n - 8:2 * n - 8])):
+        with pytest.raises(ValueError, match="shares memory"):
+            mm(r, o)
+    flat = fresh().flatten()
+    with pytest.raises(ValueError, match="shares memory"):
+        mm(flat[:m * n].view(m, n), flat[n // 2:n // 2 + m * n].view(m, n))
+    if m > 1:                                    # rows below the residual's, and one buffer in two strides
+        for r, o in ((b[:m, :n], b[1:m + 1, :n]), (flat[:m * n].view(m, n), flat[:m * 2 * n].view(m, 2 * n)[:, :n])):
+            with pytest.raises(ValueError, match="shares memory"):
+                mm(r, o)
+    raw = torch.zeros(4 * m * n + 4 * n, dtype=torch.uint8, device="cuda")
+    raw[:m * k] = ac.flatten()
+    codes, over = raw[:m * k].view(m, k), raw[:2 * m * n].view(torch.bfloat16).view(m, n)
+    with pytest.raises(ValueError, match="shares memory"):
+        fp8_block.mm(codes, bc, asc, bsc, out=over)
+    with pytest.raises(ValueError, match="shares memory"):
+        mm(None, over, raw[:4 * n].view(torch.float32))
