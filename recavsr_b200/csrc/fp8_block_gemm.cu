@@ -476,7 +476,11 @@ tile_kernel(const __grid_constant__ Maps maps, const Params p) {
           }
           if (!p.staged && res) copy_in(0);
         }
-        if (!__all_sync(0xffffffffu, wait(&acc_full[as], parity, 4))) break;
+        if (!__all_sync(0xffffffffu, wait(&acc_full[as], parity, 4))) {
+          // Given up; the residual on its way into the box lands before the CTA leaves.
+          if (inside && p.staged && res && lane == 0) sm100::mbar_wait(&res_full[w], res_phase);
+          break;
+        }
         sm100::tc_fence_after();
         uint32_t acc[64];
         load_acc(tacc + part * 64, acc);
