@@ -192,7 +192,7 @@ class DecoderSession:
         qkv_n = dim + 2 * self.hk * HEAD_DIM
         t4 = 4 * n
         e = lambda *s, dt=bf: torch.empty(s, dtype=dt, device=dev)
-        self.x, self.hr, self.xn = e(n, dim), e(t4, dim), e(t4, dim)
+        self.x, self.hr = e(n, dim), e(t4, dim)
         self.qkv, self.q_rot, self.att = e(t4, qkv_n), e(t4, dim), e(t4, dim)
         self.act = e(t4, self.hidden)
         if self.fp8:
@@ -201,6 +201,8 @@ class DecoderSession:
             self.rows8, self.rows8_s = e(t4, dim, dt=u8), e(scale_numel(t4, dim), dt=u8)
             self.act8, self.act8_s = e(t4, self.hidden, dt=u8), e(scale_numel(t4, self.hidden), dt=u8)
             self.delta = e(t4, dim)
+        else:
+            self.xn = e(t4, dim)
         self.s2 = e(t4, 768)
         self.lat_in, self.unsh, self.feats = e(n, 64), e(t4, 768), e(t4, 48)
         self.grouped, self.late_in = e(n, 192), e(t4, 64)

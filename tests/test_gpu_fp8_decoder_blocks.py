@@ -170,3 +170,9 @@ def test_planted_faults_are_refused(monkeypatch):
                     patch.setattr(o8, "values", lambda w, _: w)
                     with pytest.raises(AssertionError):
                         check(params)
+
+
+def test_buffers_are_those_of_the_linears():
+    """Neither form of the session holds the other one's activation buffers."""
+    fp8, bf16 = _session("s", linears="fp8_block"), _session("s")
+    assert not hasattr(fp8, "xn") and not hasattr(bf16, "rows8") and not hasattr(bf16, "delta")
