@@ -52,7 +52,8 @@ def dequantize(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
     """The fp32 values [rows, cols] that codes and scales stand for."""
     rows, cols = codes.shape
     e = scale_bytes(scales, rows, cols).to(torch.int32)
-    power = torch.where(e == 255, torch.nan, (e << 23).view(torch.float32))
+    power = torch.where(e == 0, 1 << 22, e << 23).view(torch.float32)      # 2^-127 is a subnormal
+    power = torch.where(e == 255, torch.nan, power)
     values = codes.view(torch.float8_e4m3fn).to(torch.float32)
     return values * power.repeat_interleave(BLOCK, 1)[:, :cols]
 
