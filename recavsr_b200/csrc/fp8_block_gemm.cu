@@ -707,7 +707,7 @@ __device__ __forceinline__ void store_piece(const Params& p, int row, int n, con
 // one warp per row, four columns per lane. SWIGLU runs a gate and an up tile
 // side by side (kW = 2): a row's 128 outputs are one warp's, so the block's
 // amax is one warp reduction. Measured: 1 x 3072 x 3072 4.0 us (2.35 TB/s of
-// weight), 24 x 3072 x 14336 11.0 us (4.1 TB/s), 1 x 512 x 512 2.8 us; bound by
+// weight), 24 x 3072 x 14336 11.0 us (4.1 TB/s), 1 x 512 x 512 2.6 us; bound by
 // the launch and the round trips before and after a CTA's k-tiles (4, 14 and 1 here).
 constexpr int kRowsThreads = 192;     // producer, MMA issuer, 4 TMEM warps; all 6 in the epilogue
 
@@ -728,8 +728,10 @@ struct RowsSmem {
   static_assert(kTotal <= 232448, "shared memory");
 };
 
+// (The bounds' second argument tells the register allocator how many CTAs share an
+// SM anyway; without it 24 x 3072 x 14336 takes 11.8 us, not 11.0.)
 template <int BT, int EPI, typename Out>
-__global__ void __launch_bounds__(kRowsThreads)
+__global__ void __launch_bounds__(kRowsThreads, RowsSmem<BT, EPI>::kPerSm)
 rows_kernel(const __grid_constant__ Maps maps, const Params p, int split) {
   using S = RowsSmem<BT, EPI>;
   constexpr int kW = S::kW, STAGES = S::kStages;
@@ -760,7 +762,7 @@ rows_kernel(const __grid_constant__ Maps maps, const Params p, int split) {
   }
   sm100::tc_fence_before();
   __syncthreads();
-  sm100::cluster_arrive();      // this CTA runs; waited for before the first store into a peer
+  sm100::cluster_arrive_relaxed();   // this CTA runs; waited for before the first store into a peer
   sm100::tc_fence_after();
   rc::pdl_trigger();
   rc::pdl_wait();
@@ -837,6 +839,9 @@ rows_kernel(const __grid_constant__ Maps maps, const Params p, int split) {
     }
   }
   __syncwarp();
+  // Every CTA of the cluster runs: their shared memory may be written. The TMEM
+  // warps are here at once, so the barrier's latency is behind the main loop.
+  sm100::cluster_wait();
   const int rows = p.M, per = (rows + split - 1) / split;       // at most BT; rank q owns rows q * per ...
   float* part = reinterpret_cast<float*>(smem + S::offPart);    // [rank][kW][per][128]
   bool ok = true;
@@ -844,7 +849,6 @@ rows_kernel(const __grid_constant__ Maps maps, const Params p, int split) {
     ok = __all_sync(0xffffffffu, wait(acc_full, 0, 13));
     sm100::tc_fence_after();
   }
-  sm100::cluster_wait();        // every CTA of the cluster runs: their shared memory may be written
   if (warp >= 2 && ok) {
     const int quad = warp & 3;
     constexpr int kChunk = BT < 32 ? BT : 32;

@@ -396,10 +396,12 @@ __device__ __forceinline__ uint32_t mapa(uint32_t saddr, uint32_t rank) {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// The two halves of cluster_sync, for work between them. Another CTA's shared
-// memory may be accessed once that CTA is known to run: after the wait.
-__device__ __forceinline__ void cluster_arrive() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+// A cluster barrier in two halves, for work between them: after the wait every CTA
+// of the cluster is known to run, and its shared memory may be accessed. Orders no
+// memory operations of the threads before the arrive (a release at cluster scope
+// would wait for them).
+__device__ __forceinline__ void cluster_arrive_relaxed() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void cluster_wait() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
