@@ -4,8 +4,10 @@
 // once, and the scale of a block comes out of the registers of the 16 lanes
 // that hold it. Measured (B200, device time, of the measured 6456 GB/s):
 // rows 7040 x 14336 bf16 52.4 us = 0.90, 14080 x 512 bf16 4.0 us = 0.84 (from
-// L2); norm with residual 14081 x 2048 fp32 57.7 us = 1.0, 3520 x 512 bf16 3.2
-// us, one row 2.2 us (launch and one round trip to memory).
+// L2); weights 14336 x 3072 fp32 33.3 us = 1.0, bf16 31.6 us = 0.65 (half the
+// bytes in flight); norm with residual 14081 x 2048 fp32 57.7 us = 1.0, 3520 x 512
+// bf16 3.2 us, one row 2.2 us (launch and one round trip to memory), 7040 x 14336
+// bf16 161 us = 0.68 (wide 16-bit rows wait for loads that stand behind stores).
 #include <type_traits>
 
 #include "fp8_block.cuh"

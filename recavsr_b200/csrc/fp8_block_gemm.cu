@@ -23,7 +23,7 @@
 // Measured (B200, device time): 7040 x 3072 x 14336 + bias + residual 240-255
 // us = 2.43-2.59 PFLOP/s, 0.72-0.77 of twice the measured bf16 rate, 274 us in a
 // loop of seconds (the 1000 W cap holds the clock at 1.25 GHz); 1759 x 3072 x
-// 3072 18.1 us; 3520 x 768 x 512 5.0 us; gated 14080 x 2048 x 512 33.0 us. What bounds
+// 3072 18.1 us; 3520 x 768 x 512 5.0 us; gated 14080 x 2048 x 512 33.1 us. What bounds
 // them: 64 (256 x 256 tiles) to 128 (128 x 128) operand bytes per clock and SM
 // that the MMAs take from L2, then the power cap; at short K the hand-over of
 // the 256-column accumulator (a tile of CTA pairs at K = 512 takes 3100-3700
